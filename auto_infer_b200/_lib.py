@@ -43,6 +43,9 @@ SIGNATURES = {
     "b200_reshape_and_cache": (c_int, [
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
         c_int, c_int, c_int, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p]),
+    "b200_reshape_and_cache_fp8": (c_int, [
+        c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+        c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
     "b200_decode_plan_bytes": (c_size_t, [c_int, c_int, c_int]),
     "b200_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "b200_decode_plan": (c_int, [

@@ -7,7 +7,7 @@
 #include <mutex>
 #include <vector>
 
-#include "common.cuh"
+#include "fp8.cuh"
 
 namespace b200 {
 
@@ -160,6 +160,31 @@ int get_query_tensor_map(const void* q, int num_tokens, int heads, int64_t token
     entries.push_back(QMapEntry{key, map});
   }
   *out = map;
+  return B200_OK;
+}
+
+// Encoded per call (a host-side packing of a few words): a map kept by address would have to be
+// told apart from that of a later cache at the same address.
+int get_fp8_cache_tensor_map(const void* cache, int num_blocks, int block_size, int heads, int box_tokens,
+                             CUtensorMap* out) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) {
+    set_last_error("cuTensorMapEncodeTiled is not available from this driver");
+    return B200_ECUDA;
+  }
+  // innermost first: dim, head, token-in-block, block
+  cuuint64_t dims[4] = {kFp8HeadDim, (cuuint64_t)heads, (cuuint64_t)block_size, (cuuint64_t)num_blocks};
+  cuuint64_t strides[3] = {kFp8HeadDim, (cuuint64_t)heads * kFp8HeadDim, (cuuint64_t)block_size * heads * kFp8HeadDim};
+  cuuint32_t box[4] = {kFp8HeadDim, 1, (cuuint32_t)box_tokens, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(cache), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_last_error("cuTensorMapEncodeTiled failed with CUresult %d (8-bit cache: blocks=%d bs=%d heads=%d)", (int)r,
+                   num_blocks, block_size, heads);
+    return B200_ECUDA;
+  }
   return B200_OK;
 }
 

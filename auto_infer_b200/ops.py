@@ -122,6 +122,69 @@ def reshape_and_cache(key: torch.Tensor, value: Optional[torch.Tensor],
 
 
 # --------------------------------------------------------------------------- #
+def _check_fp8_cache(key_cache, value_cache, key_scale, value_scale) -> tuple:
+    """(num_blocks, block_size, Hkv, D) of an 8-bit cache whose four tensors fit together."""
+    if key_cache.dtype != torch.float8_e4m3fn or value_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError("8-bit KV caches hold torch.float8_e4m3fn codes")
+    if key_scale.dtype != torch.float32 or value_scale.dtype != torch.float32:
+        raise ValueError("the scales of an 8-bit KV cache are torch.float32")
+    shape = key_cache.shape
+    if len(shape) != 4 or value_cache.shape != shape:
+        raise ValueError("8-bit KV caches must both be (num_blocks, block_size, Hkv, D)")
+    if key_scale.shape != (shape[0], shape[2]) or value_scale.shape != (shape[0], shape[2]):
+        raise ValueError("the scales of an 8-bit KV cache must be (num_blocks, Hkv)")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()
+            and key_scale.is_contiguous() and value_scale.is_contiguous()):
+        raise ValueError("8-bit KV caches and their scales must be contiguous")
+    return tuple(shape)
+
+
+def _same_device(device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"all tensors of a call must be on one device: {device} and {t.device}")
+
+
+def _aligned_rows(x: torch.Tensor, row: int) -> torch.Tensor:
+    """``x`` (T, heads, D) with its heads contiguous, tokens a multiple of 16 bytes apart and a
+    16-byte aligned base: itself when it is so already, else a copy."""
+    if (x.stride(2) != 1 or x.stride(1) != x.shape[2] or x.stride(0) % 8 or x.stride(0) < row
+            or x.data_ptr() % 16):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def reshape_and_cache_fp8(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                          value_cache: torch.Tensor, key_scale: torch.Tensor, value_scale: torch.Tensor,
+                          slot_mapping: torch.Tensor) -> None:
+    """``reshape_and_cache`` into an 8-bit cache: bf16 rows key / value (T, Hkv, 128) become e4m3
+    codes in key_cache / value_cache (num_blocks, block_size, Hkv, 128) under the power-of-two
+    scales key_scale / value_scale (num_blocks, Hkv).  A page whose first row is written starts
+    anew; otherwise its scale only grows, and its other rows are then rounded to the new scale."""
+    _need_cuda(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
+    num_blocks, block_size, n_kv, d = _check_fp8_cache(key_cache, value_cache, key_scale, value_scale)
+    _same_device(key.device, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
+    if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
+        raise ValueError("key and value rows must be torch.bfloat16")
+    t = key.shape[0]
+    if key.shape != (t, n_kv, d) or value.shape != (t, n_kv, d):
+        raise ValueError(f"key and value must be (T, {n_kv}, {d}) for this cache")
+    if slot_mapping.shape != (t,):
+        raise ValueError("slot_mapping must have one slot per token")
+    if t == 0:
+        return
+    key, value = _aligned_rows(key, n_kv * d), _aligned_rows(value, n_kv * d)
+    if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.to(torch.int32).contiguous()
+    with _on_device(key.device):
+        rc = _lib.load().b200_reshape_and_cache_fp8(
+            key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), key_cache.data_ptr(),
+            value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), slot_mapping.data_ptr(),
+            t, n_kv, d, block_size, num_blocks, status_word(key.device).data_ptr(), _stream_ptr(key.device))
+    _lib.check(rc, "b200_reshape_and_cache_fp8")
+
+
+# --------------------------------------------------------------------------- #
 class DecodePlan:
     """Host plan + device copy + workspace for one step of split-KV decode.
     Built once per step from the two host length lists and shared by all layers

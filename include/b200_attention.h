@@ -14,6 +14,7 @@
  * backends call, plus the pieces a split / context-parallel run needs:
  *
  *   b200_reshape_and_cache      auto_infer/layers/attention/base.py:41-45   (write_kv)
+ *   b200_reshape_and_cache_fp8  the same into an 8-bit cache, which the reference does not have
  *   b200_paged_decode_gqa       auto_infer/layers/attention/base.py:48-61   (paged_fia, q_len*group <= 16)
  *   b200_paged_prefill_gqa      auto_infer/layers/attention/base.py:48-61   (paged_fia, any q_len)
  *   b200_mla_decode_absorbed    auto_infer/layers/attention/mla.py:115-120  (paged_fia over the 576-wide latent)
@@ -71,6 +72,39 @@ int b200_reshape_and_cache(const void* key, const void* value,
                            int64_t key_stride, int64_t value_stride,
                            int block_size, int num_blocks,
                            int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------ *
+ * 8-bit paged cache: K and V as e4m3 codes with one fp32 scale per (page, kv
+ * head), K and V apart; a cached value is code * scale.  (No counterpart in the
+ * reference, whose caches are bf16: half the bytes a decode step reads, twice the
+ * context a GPU holds.)
+ *   key_cache / value_cache (num_blocks, block_size, Hkv, 128) e4m3, contiguous,
+ *       16-byte aligned; block_size a power of two from 16 to 1024
+ *   key_scale / value_scale (num_blocks, Hkv) fp32, contiguous
+ *
+ * Slot write, the 8-bit form of b200_reshape_and_cache: the call's rows are
+ * quantised into their slots.  Per page, head, and K and V apart: the scale the
+ * call asks for is the smallest power of two s (>= 2^-126) with |x| <= 448 s for
+ * every finite element of its rows in the page.  A page whose first row is written
+ * starts anew with that scale, and so does one whose scale is not a positive finite
+ * number (a zero-filled new pool); any other page keeps the larger of it and its
+ * own, and when the scale grows its other rows are rounded to it again.  A row's
+ * codes are x / s rounded to nearest even, infinities and NaN become NaN.
+ *   key / value (T, Hkv, 128) bf16, token strides key_stride / value_stride
+ *       elements (multiples of 8, 16-byte aligned bases)
+ *   slot_mapping (T,) int32 as b200_reshape_and_cache: any order; of equal slots the
+ *       last row is kept; negative: skipped; past the pool: B200_STATUS_BAD_SLOT.
+ * Rows of touched pages that are neither written nor re-rounded, and all other
+ * pages, keep their bytes.  The launch depends on num_tokens only and can be
+ * recorded and replayed. */
+int b200_reshape_and_cache_fp8(const void* key, int64_t key_stride,
+                               const void* value, int64_t value_stride,
+                               void* key_cache, void* value_cache,
+                               float* key_scale, float* value_scale,
+                               const int32_t* slot_mapping,
+                               int num_tokens, int num_kv_heads, int head_dim,
+                               int block_size, int num_blocks,
+                               int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------ *
  * Split-KV decode plan (host).  The reference hands the vendor op two host

@@ -384,3 +384,47 @@ def mla_paged_block(x, w, prefix, *, num_heads, qk_nope, qk_rope, v_head_dim, kv
 
 def softmax_scale_default(head_dim):
     return 1.0 / math.sqrt(head_dim)
+
+
+# --------------------------------------------------------------------------- #
+# 8-bit paged cache (no counterpart in the reference; from the definition, in 64 bits)
+# --------------------------------------------------------------------------- #
+def e4m3_round(x):
+    """Nearest e4m3 value of ``x`` (float64), ties to even: 4 significant bits from 2^-6 up, steps
+    of 2^-9 below, magnitudes past 448 (and infinities, NaN) become NaN."""
+    x = x.double()
+    e = torch.frexp(x.abs().clamp_min(2.0 ** -6)).exponent - 1
+    step = torch.ldexp(torch.ones_like(x), e - 3)
+    y = torch.round(x / step) * step
+    return torch.where(y.abs() <= 448.0, y, torch.full_like(y, math.nan))
+
+
+def fp8_scale_of(top):
+    """Smallest power of two s >= 2^-126 with top <= 448 s."""
+    s = 2.0 ** -126
+    while top > 448.0 * s:
+        s *= 2.0
+    return s
+
+
+def write_kv_fp8(rows, cache, scale, slots):
+    """One of K / V: ``rows`` (T, Hkv, D) into ``cache`` (num_blocks, block_size, Hkv, D) holding the
+    codes' values in float64, ``scale`` (num_blocks, Hkv) in float64; both updated in place.
+    Later rows win when slots repeat; negative slots and slots past the pool are skipped."""
+    num_blocks, bs, n_kv, _ = cache.shape
+    by_page = {}
+    for t, slot in enumerate(slots):
+        if 0 <= slot < num_blocks * bs:
+            by_page.setdefault(slot // bs, {})[slot % bs] = t
+    for page, taken in by_page.items():
+        for h in range(n_kv):
+            x = rows[list(taken.values()), h].double()
+            finite = x[torch.isfinite(x)].abs()
+            call = fp8_scale_of(float(finite.max()) if finite.numel() else 0.0)
+            old = float(scale[page, h])
+            anew = 0 in taken or not (0.0 < old < math.inf)
+            s = call if anew else max(old, call)
+            if not anew and s > old:
+                cache[page, :, h] = e4m3_round(cache[page, :, h] * (old / s))
+            cache[page, list(taken), h] = e4m3_round(x / s)
+            scale[page, h] = s

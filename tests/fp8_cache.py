@@ -1,0 +1,72 @@
+"""Test helper: 8-bit paged caches with shuffled pages, and their values in 64 bits."""
+import torch
+
+from oracle import paged_attention_oracle as orc
+
+E4M3 = torch.float8_e4m3fn
+
+
+def as_values(codes):
+    """The numbers e4m3 codes stand for, float64 on the CPU."""
+    return codes.cpu().float().double()
+
+
+def empty_pool(blocks, bs, n_kv, fill_byte=0, scale=0.0, d=128):
+    codes = torch.full((blocks, bs, n_kv, d), fill_byte, dtype=torch.uint8).view(E4M3)
+    return codes, torch.full((blocks, n_kv), scale, dtype=torch.float32)
+
+
+def random_pool(g, blocks, bs, n_kv, d=128, spread=1.0, any_scale=False):
+    """Codes of random rows under page scales that vary by 2^(+-spread) or so; ``any_scale``: the
+    scales are not powers of two."""
+    x = torch.randn(blocks, bs, n_kv, d, generator=g, dtype=torch.float64) * 60
+    scale = torch.exp2(torch.round(torch.randn(blocks, n_kv, generator=g) * spread) - 6)
+    if any_scale:
+        scale *= 1 + torch.rand(blocks, n_kv, generator=g)
+    return x.clamp(-448, 448).to(torch.float32).to(E4M3), scale.float()
+
+
+def deal_pages(g, lens, bs, spare=3):
+    """(number of blocks, (B, max pages) block table, flat slots of all positions in order)."""
+    need = [-(-n // bs) for n in lens]
+    blocks = sum(need) + spare
+    order = torch.randperm(blocks, generator=g)
+    table = torch.zeros(len(lens), max(need + [1]), dtype=torch.int32)
+    at, slots = 0, []
+    for b, n in enumerate(need):
+        pages = order[at:at + n]
+        table[b, :n] = pages.int()
+        at += n
+        pos = torch.arange(lens[b])
+        slots.append(pages[pos // bs] * bs + pos % bs)
+    return blocks, table, slots
+
+
+def attention(q, kc, vc, ks, vs, table, cu, kv_lens, scale, causal_base=None):
+    """softmax(scale q (k s_k)) (v s_v) per row in 64 bits: (out, lse); a row that sees no key is 0 / -inf."""
+    t, n_q, d = q.shape
+    bs, n_kv = kc.shape[1], kc.shape[2]
+    group = n_q // n_kv
+    out = torch.zeros(t, n_q, d, dtype=torch.float64)
+    lse = torch.full((t, n_q), -float("inf"), dtype=torch.float64)
+    q0 = 0
+    for b, end in enumerate(cu):
+        n, k_len = end - q0, kv_lens[b]
+        pages = table[b, :-(-k_len // bs)].long()
+        base = k_len - n if causal_base is None else causal_base[b]
+        for h in range(n_kv):
+            k = (as_values(kc[pages, :, h]) * ks[pages, h].double()[:, None, None]).reshape(-1, d)[:k_len]
+            v = (as_values(vc[pages, :, h]) * vs[pages, h].double()[:, None, None]).reshape(-1, d)[:k_len]
+            for i in range(n):
+                seen = max(0, min(base + i + 1, k_len))
+                if not seen:
+                    continue
+                heads = slice(h * group, (h + 1) * group)
+                s = q[q0 + i, heads].double() @ k[:seen].T * scale
+                lse[q0 + i, heads] = torch.logsumexp(s, -1)
+                out[q0 + i, heads] = torch.softmax(s, -1) @ v[:seen]
+        q0 = end
+    return out, lse
+
+
+__all__ = ["E4M3", "as_values", "empty_pool", "random_pool", "deal_pages", "attention", "orc"]

@@ -1,0 +1,62 @@
+"""8-bit cache: what the host refuses (no GPU needed; nothing is launched), and the oracle's rounding."""
+import math
+
+import pytest
+import torch
+
+from tests.fp8_cache import E4M3, empty_pool, orc
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from auto_infer_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+def test_oracle_rounding_agrees_with_the_type():
+    x = torch.cat([torch.linspace(-448, 448, 4001, dtype=torch.float64),
+                   torch.exp2(torch.linspace(-12, 9, 1000, dtype=torch.float64)),
+                   torch.arange(0, 256, dtype=torch.uint8).view(E4M3).double().nan_to_num(nan=0.0)])
+    x = x[x.abs() <= 448].float()
+    assert torch.equal(orc.e4m3_round(x), x.to(E4M3).double())
+    assert orc.e4m3_round(torch.tensor([math.inf, -math.inf, math.nan, 500.0])).isnan().all()
+    for top, s in ((448.0, 1.0), (449.0, 2.0), (1.75, 2.0 ** -8), (1.7500001, 2.0 ** -7), (0.0, 2.0 ** -126)):
+        assert orc.fp8_scale_of(top) == s
+
+
+def _write_args(**change):
+    a = dict(key=1 << 20, key_stride=256, value=1 << 21, value_stride=256, key_cache=1 << 22, value_cache=1 << 23,
+             key_scale=1 << 24, value_scale=1 << 25, slot_mapping=1 << 26, num_tokens=0, num_kv_heads=2, head_dim=128,
+             block_size=16, num_blocks=4, status=None, stream=None)
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(key_cache=None), -1), (dict(value_scale=None), -1), (dict(num_blocks=0), -1), (dict(num_kv_heads=0), -1),
+    (dict(num_tokens=-1), -1), (dict(num_tokens=3, slot_mapping=None), -1), (dict(num_tokens=3, key_stride=255), -1),
+    (dict(head_dim=64), -2), (dict(block_size=8), -2), (dict(block_size=24), -2), (dict(block_size=2048), -2),
+    (dict(key_cache=(1 << 22) + 8), -3), (dict(num_tokens=3, key=(1 << 20) + 8), -3),
+    (dict(num_tokens=3, value_stride=260), -3), (dict(block_size=1024, num_blocks=1 << 21), -5),
+])
+def test_slot_write_refusals(lib, change, code):
+    assert lib.b200_reshape_and_cache_fp8(*_write_args(**change)) == code
+    assert b"reshape_and_cache_fp8" in lib.b200_last_error()
+
+
+def test_empty_write_launches_nothing(lib):
+    assert lib.b200_reshape_and_cache_fp8(*_write_args()) == 0
+
+
+def test_operators_refuse_cpu_tensors_and_unfit_caches():
+    from auto_infer_b200 import ops
+    kc, ks = empty_pool(2, 16, 2)
+    rows = torch.zeros(3, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.reshape_and_cache_fp8(rows, rows, kc, kc, ks, ks, torch.zeros(3, dtype=torch.int32))
+    assert ops._check_fp8_cache(kc, kc, ks, ks) == (2, 16, 2, 128)
+    for bad in ((kc.float(), kc, ks, ks), (kc, kc[:1], ks, ks), (kc, kc, ks.double(), ks), (kc, kc, ks[:, :1], ks),
+                (kc[:, ::2], kc[:, ::2], ks, ks), (kc[0], kc[0], ks, ks)):
+        with pytest.raises(ValueError):
+            ops._check_fp8_cache(*bad)

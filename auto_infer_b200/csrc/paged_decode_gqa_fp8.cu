@@ -1,0 +1,721 @@
+// Split-KV paged GQA decode / MTP-verify attention over an 8-bit cache, for sm_100a.
+//
+//   o = sum_j softmax_j(scale * q . (ck_j s_k)) * (cv_j s_v)
+//
+// with e4m3 codes ck, cv and one scale per (page, kv head), K and V apart.  HBM-bound: a cached
+// token costs 2 * 128 bytes per kv head, half of the 16-bit cache, so an SM has half the time per
+// token for the same arithmetic.
+//
+// The plan, the work items, the TMA ring and the merge of cut pairs are those of the 16-bit kernel
+// (one persistent CTA per SM; a producer warp; two groups of four consumer warps that take alternate
+// 64-token tiles, 16 tokens a warp).  What differs:
+//   * codes become f16 on their way from shared memory to mma.sync m16n8k16: e4m3 -> f16 is exact and
+//     one instruction per pair.  Q (bf16) is scaled per row by a power of two so that it fits f16
+//     exactly, and the weights P are f16 too, three bits more than bf16.
+//   * no element is multiplied by a scale.  K's scale is uniform over a warp's 16 tokens (pages
+//     hold 16 or more) and goes into the factor that turns a product into a log2 score.  V's scale
+//     goes into the weight, w = 2^(x + log2 s_v - M): M is the running maximum of x + log2 s_v,
+//     kept beside the running maximum m of the scores x that the row sum l refers to.  So w <= 1
+//     whatever the pages' scales are, and the largest contributions have w's 11 bits.  O is in units
+//     of 2^M and is brought to l's 2^m when the row is written.
+//   * a fragment register of four codes serves two MMA k-steps (K) or two n-tiles (V): the order of
+//     the 16 dims of a k-step and of the 16 columns of an n-tile pair is free as long as Q and the
+//     output use the same, and is taken so that ldmatrix delivers the codes in place (for V after one
+//     byte permute that pairs the tokens).  A lane ends up with four neighbouring columns of O.
+//   * the scales of a tile's pages ride with the tile: 4-byte cp.async copies that complete on the
+//     stage's barrier.
+#include "decode_walk.cuh"
+#include "fp8.cuh"
+
+namespace b200 {
+
+constexpr int kF8Groups = 2;                 // consumer groups, alternate tiles
+constexpr int kF8Stages = 10;                // a multiple of the groups: a stage stays with one group for ever
+static_assert(kF8Stages % kF8Groups == 0, "each stage must always be consumed by the same warp group");
+constexpr int kF8Warps = 4 * kF8Groups;
+constexpr int kF8Consumers = kF8Warps * 32;
+constexpr int kF8Threads = kF8Consumers + 32;
+constexpr int kF8TileBytes = kTileTokens * kFp8HeadDim;          // K or V tile: 64 rows of 128 bytes
+constexpr int kF8StageBytes = 2 * kF8TileBytes;
+constexpr int kF8MaxBoxes = kTileTokens / kFp8MinBlockSize;      // pages a tile can span
+constexpr int kF8SlotFloats = kMaxRows * kHeadDim;
+static_assert(kHeadDim == kFp8HeadDim, "one head width");
+
+struct __align__(1024) DecodeFp8Smem {
+  uint8_t stage[kF8Stages][kF8StageBytes];                       // [K | V]
+  float slots[4][kF8SlotFloats];                                 // merge buffer, 4 warps at a time
+  float red_m[kF8Warps][kMaxRows];                               // running maximum of the scores
+  float red_o[kF8Warps][kMaxRows];                               // running maximum of score + log2 of V's scale
+  float red_l[kF8Warps][kMaxRows];
+  float page_scale[kF8Stages][2][kF8MaxBoxes];                   // K, V
+  uint64_t full[kF8Stages];
+  uint64_t empty[kF8Stages];
+  int abort_flag;
+  int merge_count;                                               // cut pairs whose last record this CTA wrote
+  int merge_list[kMaxDeferred];
+};
+static_assert(sizeof(DecodeFp8Smem) + 1024 <= 227 * 1024, "shared memory budget of one CTA");
+
+struct DecodeFp8Params {
+  const __nv_bfloat16* q;
+  int64_t q_stride;                 // elements between query tokens
+  const float* scale_of[2];         // (num_blocks, Hkv), K and V
+  const int32_t* block_table;
+  int64_t bt_stride;
+  int table_rows, table_cols;       // entries the table has: a plan that asks for more finds no page there
+  int num_tokens;                   // rows of q and out
+  int32_t* plan;                    // the arrival counters of its cut pairs are counted up and put back to zero
+  float* part;                      // partial records, kRecFloats each
+  void* out;                        // (T, Hq, 128) bf16 or fp32
+  float* lse_out;                   // (T, Hq) or null
+  int32_t* status;
+  int num_q_heads, num_kv_heads, group;
+  int block_size, block_shift, num_blocks;
+  int box_tokens, boxes_per_tile;
+  int out_is_f32;
+  int max_partials;                 // records the workspace holds
+  float scale_log2;
+};
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 4-byte copy to shared memory; zero when `have` is false (nothing is read then).
+__device__ __forceinline__ void cp_async_f32(float* dst, const float* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(have ? 4 : 0) : "memory");
+}
+// One of the barrier's expected arrivals, made when this thread's cp.async copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__global__ void __launch_bounds__(kF8Threads, 1)
+paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                            const DecodeFp8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  DecodeFp8Smem& sm = *reinterpret_cast<DecodeFp8Smem*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  // The plan is host-built and reaches the device by a copy, never by the kernel in
+  // front of this one: its words may be read before the grid dependency is resolved.
+  const int32_t* plan = p.plan;
+  const int4* rec = reinterpret_cast<const int4*>(plan + kPlanHeaderInts + kCtaInts * blockIdx.x);
+  const int4 r0 = __ldg(rec), r1 = __ldg(rec + 1), r2 = __ldg(rec + 2), r3 = __ldg(rec + 3);
+  const int4 hdr0 = __ldg(reinterpret_cast<const int4*>(plan));
+  const int4 hdr1 = __ldg(reinterpret_cast<const int4*>(plan) + 1);
+  const int item_begin = r0.x;
+  const int item_end = r0.y;
+  const DecodeItem* items = reinterpret_cast<const DecodeItem*>(plan + hdr1.z);   // kHdrOffItems
+
+  if (threadIdx.x == 0) {
+    sm.abort_flag = 0;
+    sm.merge_count = 0;
+    for (int s = 0; s < kF8Stages; ++s) {
+      mbar_init(&sm.full[s], 1 + p.boxes_per_tile);   // the TMA bytes, and each box's two scales
+      mbar_init(&sm.empty[s], 4);                     // one arrival per warp of the consuming group
+    }
+    mbar_fence_init();
+  }
+  __syncthreads();
+  // While the kernel in front drains: the first tiles of this CTA's first item are asked into L2 (hints
+  // only; the block ids are read past the L1 and used for nothing but the prefetch addresses).
+  if (warp == kF8Warps && item_begin < item_end) {
+    constexpr int kHintTiles = 4;
+    const int nbox = p.boxes_per_tile;
+    const int n_hint = min(r1.w - r1.z, kHintTiles) * nbox;          // tile_end - tile_begin of the first item
+    if (lane < n_hint && r2.x > 0) {
+      const int tile = r1.z + lane / nbox, box = lane % nbox;
+      int lb = ((tile * kTileTokens) >> p.block_shift) + box;
+      const int last_block = (r2.x - 1) >> p.block_shift;
+      lb = lb > last_block ? last_block : lb;
+      const bool listed = r1.x < p.table_rows && lb < p.table_cols;
+      const int bid = listed ? __ldcg(p.block_table + (int64_t)r1.x * p.bt_stride + lb) : -1;
+      if (bid >= 0 && bid < p.num_blocks) {
+        const int tok = (tile * kTileTokens + box * p.box_tokens) & (p.block_size - 1);
+        tma_prefetch_4d(&k_map, 0, r1.y, tok, bid);
+        tma_prefetch_4d(&v_map, 0, r1.y, tok, bid);
+      }
+    }
+  }
+  grid_dep_launch();              // the next kernel may be scheduled; it waits for this grid itself
+  grid_dep_wait();                // q, the block table and the step's new cache rows come from earlier kernels
+  if (hdr0.x != kPlanMagic || hdr0.y != (int)gridDim.x) {      // not a plan for this launch
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
+    return;
+  }
+  if (item_begin >= item_end) return;
+  volatile int* abort_flag = &sm.abort_flag;
+
+  if (warp == kF8Warps) {
+    // ------------------------------ producer ------------------------------
+    if (lane == 0) {
+      tma_prefetch_desc(&k_map);
+      tma_prefetch_desc(&v_map);
+    }
+    TileWalker w{items, item_begin, item_end, 0, 0, {}};
+    w.set(r1, r2, r3);
+    uint32_t it = 0;
+    const int nbox = p.boxes_per_tile;
+    // Block ids come out of a register window: lane l holds the id of logical block win_base + l of the
+    // current sequence, and the window after it is already on its way.  A tile's boxes never straddle a
+    // window (the box count divides 32).
+    int win_seq = -1, win_base = 0, win_ids = 0, nxt_ids = 0;
+    // the item after the current one is fetched when the current one starts
+    int4 na = r1, nb = r2, nc = r3;
+    auto prefetch_item = [&](int idx) {
+      if (idx < item_end) {
+        const int4* ip = reinterpret_cast<const int4*>(items + idx);
+        na = __ldg(ip); nb = __ldg(ip + 1); nc = __ldg(ip + 2);
+      }
+    };
+    prefetch_item(item_begin + 1);
+    auto load_window = [&](int seq, int base, int kv_len) -> int {
+      const int last_block = (kv_len - 1) >> p.block_shift;
+      int lb = base + lane;
+      lb = lb > last_block ? last_block : lb;         // past the end: any valid entry of the row
+      return seq < p.table_rows && lb < p.table_cols ? p.block_table[(int64_t)seq * p.bt_stride + lb] : -1;
+    };
+    while (w.item < w.item_end) {
+      if (w.tile >= w.tile_end) {                    // item done (or without any tile: an empty key range)
+        ++w.item;
+        if (w.item < w.item_end) {
+          w.set(na, nb, nc);
+          prefetch_item(w.item + 1);
+        }
+        continue;
+      }
+      const int first_lb = (w.tile * kTileTokens) >> p.block_shift;
+      const int base = first_lb & ~31;
+      if (w.cur.seq != win_seq || base != win_base) {
+        if (w.cur.seq == win_seq && base == win_base + 32) {
+          win_ids = nxt_ids;                          // the prefetched window
+        } else {
+          win_ids = load_window(w.cur.seq, base, w.cur.kv_len);
+        }
+        win_seq = w.cur.seq;
+        win_base = base;
+        nxt_ids = load_window(w.cur.seq, base + 32, w.cur.kv_len);   // used 32 blocks from now, if at all
+      }
+      // this lane's box of the tile (lanes >= nbox idle); tail boxes re-read the last valid page
+      const int last_block = (w.cur.kv_len - 1) >> p.block_shift;
+      int lb = first_lb + (lane < nbox ? lane : 0);
+      lb = lb > last_block ? last_block : lb;
+      int b = __shfl_sync(0xffffffffu, win_ids, lb - win_base);
+
+      const int s = it % kF8Stages;
+      const uint32_t ph = (it / kF8Stages) & 1u;
+      if (lane == 0) {
+        mbar_wait_bounded(&sm.empty[s], ph ^ 1u, abort_flag, p.status);
+        mbar_arrive_expect_tx(&sm.full[s], kF8StageBytes);
+      }
+      __syncwarp();
+      if (lane < nbox) {
+        const bool have = b >= 0 && b < p.num_blocks;
+        if (!have) {                                // out-of-pool id: codes and scales are zero, flag it
+          if (p.status) atomicOr(p.status, B200_STATUS_BAD_BLOCK);
+          b = p.num_blocks;
+        }
+        const int tok = (w.tile * kTileTokens + lane * p.box_tokens) & (p.block_size - 1);
+        uint8_t* dst = sm.stage[s] + lane * p.box_tokens * kFp8HeadDim;
+        const int h = w.cur.kv_head;
+        tma_load_4d(dst, &k_map, &sm.full[s], 0, h, tok, b);
+        tma_load_4d(dst + kF8TileBytes, &v_map, &sm.full[s], 0, h, tok, b);
+        const int64_t at = have ? (int64_t)b * p.num_kv_heads + h : 0;
+        cp_async_f32(&sm.page_scale[s][0][lane], p.scale_of[0] + at, have);
+        cp_async_f32(&sm.page_scale[s][1][lane], p.scale_of[1] + at, have);
+        cp_async_arrive(&sm.full[s]);
+      }
+      __syncwarp();
+      ++it;
+      ++w.tile;
+    }
+    // drain: do not leave while copies may still land in this CTA's shared memory
+    if (lane == 0) {
+      const uint32_t n = it < (uint32_t)kF8Stages ? it : (uint32_t)kF8Stages;
+      for (uint32_t k = 0; k < n; ++k) {
+        const uint32_t j = it - 1 - k;
+        mbar_wait_bounded(&sm.full[j % kF8Stages], (j / kF8Stages) & 1u, abort_flag, p.status);
+      }
+    }
+    return;
+  }
+
+  // -------------------------------- consumers --------------------------------
+  const int grp = warp >> 2;          // which tiles (running tile counter modulo the groups)
+  const int wslice = warp & 3;        // 16-token slice of the tile
+  const int quad = lane >> 2;         // fragment row (and row + 8)
+  const int qlane = lane & 3;
+  const int G = p.group;
+  const int box = (wslice * 16) / p.box_tokens;                          // the page of this warp's tokens
+
+  // ldmatrix lane addressing (row of the tile, which of two 16-byte chunks)
+  const int k_tok = wslice * 16 + ((lane >> 4) << 3) + (lane & 7);       // matrices 2,3 -> tokens +8
+  const int k_sel = (lane >> 3) & 1;                                     // matrices 1,3 -> next chunk
+  const int v_tok = wslice * 16 + (((lane >> 3) & 1) << 3) + (lane & 7); // matrices 1,3 -> tokens +8
+  const int v_sel = lane >> 4;                                           // matrices 2,3 -> next chunk
+
+  TileWalker w{items, item_begin, item_end, 0, 0, {}};
+  w.set(r1, r2, r3);
+  uint32_t it = 0;
+
+  // Q rows of an item as they lie in memory, 8 bytes (4 dims) per 16-dim k-step; rows beyond q_len*group
+  // are zero.  They are fetched for the NEXT item right after the tile loop, so the global loads fly
+  // while the warps merge and write the current item.
+  uint2 qraw[2][8];
+  // rows of an item; none if they do not lie within q and out (a plan refilled for a larger step)
+  auto rows_of = [&](const DecodeItem& qi) -> int {
+    return qi.q_start + qi.q_len <= p.num_tokens ? qi.q_len * G : 0;
+  };
+  auto load_q = [&](const DecodeItem& qi) {
+    const int qrows = rows_of(qi);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = quad + 8 * h;
+      const bool have = row < qrows;
+      const __nv_bfloat16* src = p.q + (int64_t)(qi.q_start + (have ? row / G : 0)) * p.q_stride +
+                                 (int64_t)(qi.kv_head * G + (have ? row % G : 0)) * kHeadDim + qlane * 4;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+        qraw[h][ks] = have ? *reinterpret_cast<const uint2*>(src + ks * 16) : make_uint2(0u, 0u);
+    }
+  };
+  load_q(w.cur);
+
+  // A partial record is announced (arrival counter of its pair) one item late, or at the end
+  // of the CTA's work: by then its stores have long left the SM and the fence that must
+  // precede the announcement costs nothing.
+  int pending_multi = -1;
+  const int off_multi = hdr1.w;
+  auto announce = [&](int multi_idx) {            // thread 0, after a fence by all and a barrier
+    MultiGroup* mg = reinterpret_cast<MultiGroup*>(p.plan + off_multi) + multi_idx;
+    const int n_parts = mg->part_end - mg->part_begin;
+    if (atomicAdd(&mg->arrivals, 1) == n_parts - 1) {
+      mg->arrivals = 0;                           // ready for the next launch on this plan
+      __threadfence();                            // the other CTAs' records are visible from here on
+      if (sm.merge_count < kMaxDeferred) {
+        sm.merge_list[sm.merge_count] = multi_idx;
+        sm.merge_count = sm.merge_count + 1;
+      } else if (p.status) {                      // the planner never gives a CTA this many cut pieces
+        atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
+      }
+    }
+  };
+  // the record of the item after the current one, fetched while the current one streams
+  int4 na = r1, nb = r2;
+  auto prefetch_item = [&](int idx) {
+    if (idx < item_end) {
+      const int4* ip = reinterpret_cast<const int4*>(items + idx);
+      na = __ldg(ip); nb = __ldg(ip + 1);
+    }
+  };
+  prefetch_item(item_begin + 1);
+
+  while (w.item < w.item_end) {
+    const DecodeItem item = w.cur;
+    const int rows = rows_of(item);
+    // last visible key per fragment row (-1: row unused, everything masked)
+    const int lim[2] = {quad < rows ? min(item.causal_base + quad / G, item.kv_len - 1) : -1,
+                        quad + 8 < rows ? min(item.causal_base + (quad + 8) / G, item.kv_len - 1) : -1};
+
+    // ---- Q to f16: each row times a power of two that brings its largest magnitude to [2^14, 2^15).
+    // bf16 has 8 significant bits, f16 11 down to 2^-14: exact for all elements within 2^-28 of the
+    // row's largest, and 2^-39 of it off at most below that.
+    uint32_t qf[8][4];
+    float to_log2[2];                  // what turns a product of the row with K codes into units of log2 / s_k
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        top = max(top, max(qraw[h][ks].x & 0x7fffu, (qraw[h][ks].x >> 16) & 0x7fffu));
+        top = max(top, max(qraw[h][ks].y & 0x7fffu, (qraw[h][ks].y >> 16) & 0x7fffu));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = max((int)(top >> 7), 15);                      // exponent field; at least 15 keeps both factors normal
+      const float up = __uint_as_float((uint32_t)(268 - e) << 23); // 2^(14 - (e - 127))
+      to_log2[h] = __uint_as_float((uint32_t)(e - 14) << 23) * p.scale_log2;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        const uint2 v = qraw[h][ks];
+        qf[ks][h] = pack_f16(__uint_as_float(v.x << 16) * up, __uint_as_float(v.x & 0xffff0000u) * up);
+        qf[ks][2 + h] = pack_f16(__uint_as_float(v.y << 16) * up, __uint_as_float(v.y & 0xffff0000u) * up);
+      }
+    }
+
+    float o[16][4];                    // [16-column chunk * 2 + even / odd column][fragment]
+#pragma unroll
+    for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, mo[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int tile = item.tile_begin; tile < item.tile_end; ++tile, ++it) {
+      if ((int)(it % kF8Groups) != grp) continue;
+      const int s = it % kF8Stages;
+      mbar_wait_bounded(&sm.full[s], (it / kF8Stages) & 1u, abort_flag, p.status);
+      const uint32_t kbase = smem_u32(sm.stage[s]);
+      const uint32_t vbase = kbase + kF8TileBytes;
+      const float s_k = sm.page_scale[s][0][box], s_v = sm.page_scale[s][1][box];
+
+      // ---- S = Q K^T for this warp's 16 tokens (two n-tiles of 8); four accumulator sets shorten the
+      // chain of dependent MMAs
+      float sacc[2][2][4];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) sacc[c][n][0] = sacc[c][n][1] = sacc[c][n][2] = sacc[c][n][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t kb[4];
+        ldmatrix_x4(kb, kbase + swz128(k_tok, j * 2 + k_sel));
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint32_t codes = kb[n * 2 + c];
+            mma_f16_16816(sacc[c][n], qf[j * 2 + c], e4m3x2_to_f16x2((uint16_t)codes),
+                          e4m3x2_to_f16x2((uint16_t)(codes >> 16)));
+          }
+      }
+      // ---- mask + online softmax (fp32, exp2 domain)
+      const int tok0 = tile * kTileTokens + wslice * 16 + qlane * 2;
+      const float lv = fast_log2(s_v);
+      float x[2][4];                   // [row][n-tile * 2 + e]
+      float w_of[2];                   // what turns p = 2^(x - m) into the weight 2^(x + lv - mo)
+      bool grown = false;
+      float shrink_o[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float f = to_log2[h] * s_k;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float y = (sacc[0][n][2 * h + e] + sacc[1][n][2 * h + e]) * f;
+            if (tok0 + n * 8 + e > lim[h]) y = -INFINITY;
+            x[h][n * 2 + e] = y;
+            mx = fmaxf(mx, y);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m[h], mx);
+        const float ms = m_new == -INFINITY ? 0.f : m_new;
+        l[h] *= fast_exp2(m[h] - ms);                              // m = -inf -> 0
+        m[h] = m_new;
+        const float mo_new = fmaxf(mo[h], mx + lv);
+        const float mos = mo_new == -INFINITY ? 0.f : mo_new;
+        shrink_o[h] = fast_exp2(mo[h] - mos);
+        grown |= mo_new != mo[h];
+        mo[h] = mo_new;
+        // bounded, so that a weight whose p is 0 does not become 0 * inf (a NaN scale stays NaN)
+        const float up = m_new + lv - mos;
+        w_of[h] = fast_exp2(up > 126.f ? 126.f : up);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[h][i] = fast_exp2(x[h][i] - ms);
+          l[h] += x[h][i];
+        }
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          o[n][0] *= shrink_o[0]; o[n][1] *= shrink_o[0]; o[n][2] *= shrink_o[1]; o[n][3] *= shrink_o[1];
+        }
+      }
+      uint32_t pf[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          pf[n * 2 + h] = pack_f16(x[h][n * 2] * w_of[h], x[h][n * 2 + 1] * w_of[h]);
+      // ---- rows past the sequence's end carry weight 0, but 0 x NaN is NaN: whatever codes an
+      // unwritten cache slot holds must not reach the MMA.  Only a pair's last tile has such rows;
+      // the warp clears its own 16 of them in shared memory.
+      const bool ragged = (tile + 1) * kTileTokens > item.kv_len;
+      if (ragged) {
+        const int first_bad = item.kv_len - tile * kTileTokens;          // first row of the tile past the end
+        for (int idx = lane; idx < 16 * 8; idx += 32) {
+          const int row = wslice * 16 + (idx >> 3);
+          if (row >= first_bad)
+            *reinterpret_cast<uint4*>(sm.stage[s] + kF8TileBytes + swz128(row, idx & 7)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+      }
+      // ---- O += P V (k = this warp's 16 tokens, n = 128 dims)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t vb[4];
+        ldmatrix_x4_trans(vb, vbase + swz128(v_tok, j * 2 + v_sel));
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          // bytes (token, column): (t0,d0) (t0,d1) (t1,d0) (t1,d1) -> column d0's tokens, column d1's tokens
+          const uint32_t lo = __byte_perm(vb[c * 2], 0, 0x3120), hi = __byte_perm(vb[c * 2 + 1], 0, 0x3120);
+          const int n = (j * 2 + c) * 2;
+          mma_f16_16816(o[n], pf, e4m3x2_to_f16x2((uint16_t)lo), e4m3x2_to_f16x2((uint16_t)hi));
+          mma_f16_16816(o[n + 1], pf, e4m3x2_to_f16x2((uint16_t)(lo >> 16)), e4m3x2_to_f16x2((uint16_t)(hi >> 16)));
+        }
+      }
+      // the stage goes back to TMA: order this warp's stores into it before TMA's writes
+      if (ragged) fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[s]);
+    }
+
+    // ---- next item's Q on its way, then merge the warps (fixed order) and write the result
+    ++w.item;
+    if (w.item < w.item_end) {
+      w.set(na, nb, __ldg(reinterpret_cast<const int4*>(items + w.item) + 2));
+      prefetch_item(w.item + 1);
+      load_q(w.cur);
+    }
+    if (pending_multi >= 0) __threadfence();      // stores of the PREVIOUS partial record (long done)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (qlane == 0) {
+        sm.red_m[warp][quad + 8 * h] = m[h];
+        sm.red_o[warp][quad + 8 * h] = mo[h];
+      }
+    }
+    named_bar_sync(1, kF8Consumers);                           // (1) every warp's row maxima are in place
+    if (pending_multi >= 0) {
+      if (threadIdx.x == 0) announce(pending_multi);
+      pending_multi = -1;
+    }
+    // bring this warp's sums and accumulators to the rows' common maxima
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float g = -INFINITY, go = -INFINITY;
+#pragma unroll
+      for (int ww = 0; ww < kF8Warps; ++ww) {
+        g = fmaxf(g, sm.red_m[ww][quad + 8 * h]);
+        go = fmaxf(go, sm.red_o[ww][quad + 8 * h]);
+      }
+      const float f = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - g);
+      const float fo = mo[h] == -INFINITY ? 0.f : fast_exp2(mo[h] - go);
+      if (qlane == 0) sm.red_l[warp][quad + 8 * h] = l[h] * f;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        o[n][2 * h] *= fo;
+        o[n][2 * h + 1] *= fo;
+      }
+    }
+    // A lane holds four neighbouring columns of a row: 16-byte accesses, of which the eight lanes of a
+    // phase belong to two rows.  Rows are a multiple of the 32 banks apart, so odd rows have their
+    // 16-column halves swapped.
+    const int swz = (quad & 1) << 4;              // same for row quad and row quad + 8
+    if (warp >= 4 && warp < 8) {
+      float* slot = sm.slots[warp - 4];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const int col = (c * 16 + qlane * 4) ^ swz;
+        *reinterpret_cast<float4*>(slot + quad * kHeadDim + col) =
+            make_float4(o[2 * c][0], o[2 * c + 1][0], o[2 * c][1], o[2 * c + 1][1]);
+        *reinterpret_cast<float4*>(slot + (quad + 8) * kHeadDim + col) =
+            make_float4(o[2 * c][2], o[2 * c + 1][2], o[2 * c][3], o[2 * c + 1][3]);
+      }
+    }
+    named_bar_sync(1, kF8Consumers);                           // (2) warps 4-7 have parked their sums
+    if (warp < 4) {
+      // Add the partner warp's sums in place: a thread rewrites exactly the words it read.  Loads of four
+      // chunks are issued together before any of their stores (the compiler must assume they alias).
+      float* slot = sm.slots[warp];
+#pragma unroll
+      for (int c0 = 0; c0 < 8; c0 += 4) {
+        float4 a[4], b[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int col = ((c0 + u) * 16 + qlane * 4) ^ swz;
+          a[u] = *reinterpret_cast<const float4*>(slot + quad * kHeadDim + col);
+          b[u] = *reinterpret_cast<const float4*>(slot + (quad + 8) * kHeadDim + col);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c = c0 + u, col = (c * 16 + qlane * 4) ^ swz;
+          *reinterpret_cast<float4*>(slot + quad * kHeadDim + col) =
+              make_float4(a[u].x + o[2 * c][0], a[u].y + o[2 * c + 1][0], a[u].z + o[2 * c][1], a[u].w + o[2 * c + 1][1]);
+          *reinterpret_cast<float4*>(slot + (quad + 8) * kHeadDim + col) =
+              make_float4(b[u].x + o[2 * c][2], b[u].y + o[2 * c + 1][2], b[u].z + o[2 * c][3], b[u].w + o[2 * c + 1][3]);
+        }
+      }
+    }
+    // 256 threads: thread -> rows (t / 32) and (t / 32 + 8), 4 columns each, so a warp reads and
+    // writes whole rows.  The rows' maxima and scaled sums are taken BEFORE barrier (3): no warp
+    // writes those arrays again (next item) until every thread has passed (3).
+    const int t = threadIdx.x;
+    const int col = (t & 31) * 4;
+    float inv_r[2], unit_r[2], lse_r[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = (t >> 5) + h * 8;
+      float g = -INFINITY, go = -INFINITY, lsum = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < kF8Warps; ++ww) {
+        g = fmaxf(g, sm.red_m[ww][row]);
+        go = fmaxf(go, sm.red_o[ww][row]);
+        lsum += sm.red_l[ww][row];
+      }
+      // O is in units of 2^go, the sum in units of 2^g; the factor between them in two halves, each of
+      // which fp32 holds however far apart they are
+      inv_r[h] = lsum > 0.f ? 1.f / lsum : 0.f;
+      unit_r[h] = go == -INFINITY ? 0.f : fast_exp2((go - g) * 0.5f);
+      lse_r[h] = lsum > 0.f ? g * 0.6931471805599453f + __logf(lsum) : -INFINITY;
+    }
+    named_bar_sync(1, kF8Consumers);                           // (3) the four slots hold the warp-pair sums
+    const bool record_fits = (item.direct || item.partial_idx < p.max_partials) && rows > 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = (t >> 5) + h * 8;
+      if (row >= rows || !record_fits) continue;
+      const int pcol = col ^ ((row & 1) << 4);
+      float4 acc = *reinterpret_cast<const float4*>(&sm.slots[0][row * kHeadDim + pcol]);
+#pragma unroll
+      for (int sl = 1; sl < 4; ++sl) {
+        const float4 y = *reinterpret_cast<const float4*>(&sm.slots[sl][row * kHeadDim + pcol]);
+        acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+      }
+      const float u = unit_r[h], inv = inv_r[h];
+      const float4 v = make_float4(acc.x * inv * u * u, acc.y * inv * u * u, acc.z * inv * u * u, acc.w * inv * u * u);
+      if (item.direct) {
+        const int64_t tok = item.q_start + row / G;
+        const int head = item.kv_head * G + row % G;
+        const int64_t off = (tok * p.num_q_heads + head) * kHeadDim + col;
+        if (p.out_is_f32) {
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + off) = v;
+        } else {
+          uint2 pk;
+          pk.x = pack_bf16(v.x, v.y);
+          pk.y = pack_bf16(v.z, v.w);
+          *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + off) = pk;
+        }
+        if (p.lse_out && (t & 31) == 0) p.lse_out[tok * p.num_q_heads + head] = lse_r[h];
+      } else {
+        float* rec = p.part + (int64_t)item.partial_idx * kRecFloats;
+        *reinterpret_cast<float4*>(rec + row * kHeadDim + col) = v;
+        if ((t & 31) == 0) rec[kMaxRows * kHeadDim + row] = lse_r[h];
+      }
+    }
+    if (!record_fits) {                                        // workspace, q or out smaller than the plan needs
+      if (t == 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
+    } else if (!item.direct) {
+      pending_multi = item.multi_idx;
+    }
+    // The next item's first write to red_m / red_o comes after barrier (3) above, and its first write
+    // to red_l and to the slots after its own barrier (1), which no thread passes before it has
+    // finished the reads of this item.
+  }
+
+  // ---- the last record's announcement, then the merges this CTA owes: the cut pairs
+  // whose last record it wrote
+  if (pending_multi >= 0) {
+    __threadfence();
+    named_bar_sync(1, kF8Consumers);
+    if (threadIdx.x == 0) announce(pending_multi);
+  }
+  named_bar_sync(1, kF8Consumers);
+  if (sm.merge_count > 0) merge_noted_pairs(p, sm.merge_list, sm.merge_count, off_multi);
+}
+
+}  // namespace b200
+
+extern "C" int b200_paged_decode_gqa_fp8(const void* q, int64_t q_stride, const void* key_cache,
+                                         const void* value_cache, const float* key_scale,
+                                         const float* value_scale, int num_blocks, int block_size,
+                                         const int32_t* block_table, int64_t bt_stride, int table_rows,
+                                         int table_cols, int32_t* plan_dev, const b200_decode_plan_info* info,
+                                         int num_ctas, int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, float scale, void* workspace,
+                                         size_t workspace_bytes, void* out, int out_is_f32, float* lse_out,
+                                         int32_t* status, void* stream) {
+  using namespace b200;
+  const char* who = "paged_decode_gqa_fp8";
+  int rc = check_fp8_cache(who, key_cache, value_cache, key_scale, value_scale, num_blocks, block_size, num_kv_heads,
+                           head_dim);
+  if (rc) return rc;
+  if (info) num_ctas = info->num_ctas;
+  if (info && info->num_items == 0) return B200_OK;
+  if (!q || !block_table || !plan_dev || !out || !workspace || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
+      num_ctas <= 0 || num_tokens < 0 || table_rows <= 0 || table_cols <= 0) {
+    set_last_error("%s: null pointer, bad head counts, no CTAs or an empty block table", who);
+    return B200_EINVAL;
+  }
+  if (reinterpret_cast<uintptr_t>(q) % 8 || q_stride % 4 || q_stride < (int64_t)num_q_heads * head_dim) {
+    set_last_error("%s: q must be 8-byte aligned with a token stride >= Hq*D that is a multiple of 4 elements", who);
+    return B200_EALIGN;
+  }
+  if (reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+      reinterpret_cast<uintptr_t>(plan_dev) % 16) {
+    set_last_error("%s: out, workspace and plan must be 16-byte aligned", who);
+    return B200_EALIGN;
+  }
+  const size_t max_partials = workspace_bytes / (kRecFloats * sizeof(float));
+  if (info && (size_t)info->num_partials > max_partials) {
+    set_last_error("%s: workspace %zu bytes < %zu needed", who, workspace_bytes,
+                   (size_t)info->num_partials * kRecFloats * sizeof(float));
+    return B200_EPLAN;
+  }
+  const int box_tokens = block_size < kTileTokens ? block_size : kTileTokens;
+  CUtensorMap k_map, v_map;
+  rc = get_fp8_cache_tensor_map(key_cache, num_blocks, block_size, num_kv_heads, box_tokens, &k_map);
+  if (rc) return rc;
+  rc = get_fp8_cache_tensor_map(value_cache, num_blocks, block_size, num_kv_heads, box_tokens, &v_map);
+  if (rc) return rc;
+
+  DecodeFp8Params p;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride = q_stride;
+  p.scale_of[0] = key_scale;
+  p.scale_of[1] = value_scale;
+  p.block_table = block_table;
+  p.bt_stride = bt_stride;
+  p.table_rows = table_rows;
+  p.table_cols = table_cols;
+  p.num_tokens = num_tokens;
+  p.plan = plan_dev;
+  p.part = static_cast<float*>(workspace);
+  p.max_partials = max_partials > (size_t)INT32_MAX ? INT32_MAX : (int)max_partials;
+  p.out = out;
+  p.lse_out = lse_out;
+  p.status = status;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads;
+  p.block_size = block_size;
+  p.block_shift = __builtin_ctz(block_size);
+  p.num_blocks = num_blocks;
+  p.box_tokens = box_tokens;
+  p.boxes_per_tile = kTileTokens / box_tokens;
+  p.out_is_f32 = out_is_f32;
+  p.scale_log2 = scale * 1.4426950408889634f;
+
+  const size_t smem = sizeof(DecodeFp8Smem) + 1024;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_set[dev]) {
+    rc = check_cuda(cudaFuncSetAttribute(paged_decode_gqa_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem),
+                    "paged_decode_gqa_fp8 smem attribute");
+    if (rc) return rc;
+    if (dev < 64) attr_set[dev] = true;
+  }
+  return check_cuda(launch_pdl(paged_decode_gqa_fp8_kernel, dim3(num_ctas), dim3(kF8Threads), smem,
+                               static_cast<cudaStream_t>(stream), k_map, v_map, p),
+                    "paged_decode_gqa_fp8 launch");
+}

@@ -242,6 +242,8 @@ class DecodePlan:
         self.num_seqs = len(cu_seqlens_q)
         if self.num_seqs > self.capacity_seqs:
             raise ValueError(f"{self.num_seqs} sequences exceed the plan's capacity of {self.capacity_seqs}")
+        self.num_tokens = int(cu_seqlens_q[-1]) if self.num_seqs else 0
+        self.max_kv = max(seqlens_kv, default=0)
         # plain C arrays: cheaper than tensors for a few dozen integers on the per-step path
         int_array = ctypes.c_int32 * self.num_seqs
         cu = int_array(*cu_seqlens_q)
@@ -374,6 +376,63 @@ def paged_decode_gqa_write(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Te
     return out
 
 
+def _fp8_attention_args(who, q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
+                        lse_out):
+    """Checks and tensors shared by the attention calls over an 8-bit cache: (q, block_table, out, cache shape)."""
+    _need_cuda(q, key_cache, value_cache, key_scale, value_scale, block_table, out, lse_out)
+    shape = _check_fp8_cache(key_cache, value_cache, key_scale, value_scale)
+    _, block_size, n_kv, d = shape
+    _same_device(q.device, key_cache, value_cache, key_scale, value_scale, block_table, out, lse_out, plan.dev)
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != d:
+        raise ValueError(f"{who}: q must be (T, Hq, {d}) torch.bfloat16")
+    t, n_q, _ = q.shape
+    if n_q != plan.num_q_heads or n_kv != plan.num_kv_heads:
+        raise ValueError(f"{who}: the plan was built for {plan.num_q_heads} / {plan.num_kv_heads} heads, "
+                         f"the tensors have {n_q} / {n_kv}")
+    if t < plan.num_tokens:
+        raise ValueError(f"{who}: the plan covers {plan.num_tokens} query rows, q has {t}")
+    if block_table.dim() != 2 or block_table.shape[0] < plan.num_seqs or \
+            block_table.shape[1] * block_size < plan.max_kv:
+        raise ValueError(f"{who}: block_table must have {plan.num_seqs} rows of at least "
+                         f"{-(-plan.max_kv // block_size)} blocks")
+    if block_table.dtype != torch.int32:
+        block_table = block_table.to(torch.int32)
+    if block_table.numel() == 0:                     # no sequence has keys: a table to point at, never read
+        block_table = torch.zeros(1, 1, dtype=torch.int32, device=q.device)
+    elif block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    if out is None:
+        out = torch.empty(t, n_q, d, dtype=torch.float32 if out_f32 else q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype not in (torch.bfloat16, torch.float32) or not out.is_contiguous():
+        raise ValueError(f"{who}: out must be contiguous, of q's shape, torch.bfloat16 or torch.float32")
+    if lse_out is not None and (lse_out.shape != (t, n_q) or lse_out.dtype != torch.float32
+                                or not lse_out.is_contiguous()):
+        raise ValueError(f"{who}: lse_out must be contiguous (T, Hq) torch.float32")
+    return _aligned_rows(q, n_q * d), block_table, out, shape
+
+
+def paged_decode_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                         key_scale: torch.Tensor, value_scale: torch.Tensor, block_table: torch.Tensor,
+                         plan: DecodePlan, scale: float, out: Optional[torch.Tensor] = None, out_f32: bool = False,
+                         lse_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_decode_gqa`` over an 8-bit cache (see ``reshape_and_cache_fp8``): the same plans, masks
+    and outputs.  Rows of sequences the plan skipped are left untouched in ``out``."""
+    q, block_table, out, (num_blocks, block_size, n_kv, d) = _fp8_attention_args(
+        "paged_decode_gqa_fp8", q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
+        lse_out)
+    with _on_device(q.device):
+        rc = _lib.load().b200_paged_decode_gqa_fp8(
+            q.data_ptr(), q.stride(0), key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(),
+            value_scale.data_ptr(), num_blocks, block_size, block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[0], block_table.shape[1], plan.dev.data_ptr(),
+            None if plan.replayable else ctypes.byref(plan.info), plan.num_ctas, q.shape[0], q.shape[1], n_kv, d,
+            float(scale), plan.workspace.data_ptr(), plan.workspace.numel(), out.data_ptr(),
+            1 if out.dtype == torch.float32 else 0, lse_out.data_ptr() if lse_out is not None else None,
+            status_word(q.device).data_ptr(), _stream_ptr(q.device))
+    _lib.check(rc, "b200_paged_decode_gqa_fp8")
+    return out
+
+
 class MlaDecodePlan(DecodePlan):
     """Host plan + device copy + workspace of the absorbed-MLA decode kernel (32-token latent
     tiles, one shared latent head).  ``capacity_seqs`` makes it replayable like ``DecodePlan``:
@@ -481,6 +540,8 @@ class PrefillPlan:
         if num_seqs > self.capacity_seqs or num_tokens > self.capacity_tokens:
             raise ValueError(f"step of {num_seqs} sequences / {num_tokens} tokens exceeds the plan's capacity "
                              f"({self.capacity_seqs} / {self.capacity_tokens})")
+        self.num_seqs, self.num_tokens = num_seqs, num_tokens
+        self.max_kv = max(seqlens_kv, default=0)
         int_array = ctypes.c_int32 * max(num_seqs, 1)
         cu = int_array(*cu_seqlens_q)
         kv = int_array(*seqlens_kv)

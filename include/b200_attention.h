@@ -249,6 +249,31 @@ int b200_paged_decode_gqa_write(const void* q, int64_t q_stride,
                                 int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------ *
+ * The same attention over an 8-bit cache (layout and scales as
+ * b200_reshape_and_cache_fp8): o = softmax(scale q (ck s_k)) (cv s_v).  Plans,
+ * workspace, masks, q, out and lse_out as b200_paged_decode_gqa; with info == NULL
+ * the launch is the replayable one (grid num_ctas, counts read from the plan).
+ *   block_size a power of two from 16 to 1024; q 8-byte aligned, q_stride a multiple
+ *       of 4 elements
+ *   scales: positive finite numbers, any, not only powers of two
+ *   table_rows, table_cols: entries of block_table; a sequence or page past them
+ *       reads as zeros and sets B200_STATUS_BAD_BLOCK
+ *   num_tokens: rows of q and out; items of the plan past them are left out and set
+ *       B200_STATUS_BAD_LAUNCH
+ * Cache rows past a sequence's kv_len may hold any codes. */
+int b200_paged_decode_gqa_fp8(const void* q, int64_t q_stride,
+                              const void* key_cache, const void* value_cache,
+                              const float* key_scale, const float* value_scale,
+                              int num_blocks, int block_size,
+                              const int32_t* block_table, int64_t bt_stride,
+                              int table_rows, int table_cols,
+                              int32_t* plan_dev, const b200_decode_plan_info* info, int num_ctas,
+                              int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, float scale,
+                              void* workspace, size_t workspace_bytes,
+                              void* out, int out_is_f32, float* lse_out,
+                              int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------ *
  * Paged GQA attention for wide query blocks: chunked prefill over a cached
  * prefix and multi-token verify, any q_len, bottom-right causal.  Replaces
  * paged_fia (auto_infer/layers/attention/base.py:48-61) for the rows the decode

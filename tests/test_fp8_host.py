@@ -60,3 +60,27 @@ def test_operators_refuse_cpu_tensors_and_unfit_caches():
                 (kc[:, ::2], kc[:, ::2], ks, ks), (kc[0], kc[0], ks, ks)):
         with pytest.raises(ValueError):
             ops._check_fp8_cache(*bad)
+
+
+def _decode_args(**change):
+    from auto_infer_b200._lib import DecodePlanInfo
+    import ctypes
+    info = DecodePlanInfo(num_ctas=4, num_items=1, num_partials=1)
+    a = dict(q=1 << 20, q_stride=1024, key_cache=1 << 22, value_cache=1 << 23, key_scale=1 << 24, value_scale=1 << 25,
+             num_blocks=4, block_size=16, block_table=1 << 26, bt_stride=4, table_rows=1, table_cols=4, plan=1 << 27,
+             info=ctypes.byref(info), num_ctas=4, num_tokens=1, num_q_heads=8, num_kv_heads=2, head_dim=128, scale=0.1,
+             workspace=1 << 28, workspace_bytes=1 << 16, out=1 << 29, out_is_f32=0, lse_out=None, status=None, stream=None)
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(q=None), -1), (dict(block_table=None), -1), (dict(plan=None), -1), (dict(workspace=None), -1), (dict(out=None), -1),
+    (dict(key_scale=None), -1), (dict(num_q_heads=7), -1), (dict(num_tokens=-1), -1), (dict(table_rows=0), -1),
+    (dict(table_cols=0), -1), (dict(info=None, num_ctas=0), -1), (dict(head_dim=96), -2), (dict(block_size=8), -2),
+    (dict(q=(1 << 20) + 4), -3), (dict(q_stride=1022), -3), (dict(out=(1 << 29) + 8), -3), (dict(plan=(1 << 27) + 4), -3),
+    (dict(workspace_bytes=100), -6),
+])
+def test_decode_refusals(lib, change, code):
+    assert lib.b200_paged_decode_gqa_fp8(*_decode_args(**change)) == code
+    assert b"paged_decode_gqa_fp8" in lib.b200_last_error()

@@ -26,7 +26,7 @@ SOURCES = [
     "cp_exchange.cu",
     "copy_blocks.cu",
     "rope_cache.cu", "paged_mha.cu",
-    "reshape_and_cache_fp8.cu", "paged_decode_gqa_fp8.cu",
+    "reshape_and_cache_fp8.cu", "paged_decode_gqa_fp8.cu", "paged_prefill_gqa_fp8.cu",
 ]
 
 NVCC_FLAGS = [

@@ -55,5 +55,23 @@ __device__ __forceinline__ float fp8_scale_of(float a) {
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 4-byte copy to shared memory; zero when `have` is false (nothing is read then).
+__device__ __forceinline__ void cp_async_f32(float* dst, const float* src, bool have) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(have ? 4 : 0) : "memory");
+}
+// One of the barrier's expected arrivals, made when this thread's cp.async copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 #endif  // __CUDACC__
 }  // namespace b200

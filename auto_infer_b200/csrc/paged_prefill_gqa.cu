@@ -13,33 +13,13 @@
 
 #define B200_INLINE_WAITS
 #include "common.cuh"
-#include "decode_plan.h"
+#include "prefill_plan.cuh"
 #include "tc05.cuh"
 
 namespace b200 {
 
-constexpr int kPfHeadDim = 128;
-constexpr int kPfRows = 128;                                   // packed query rows per item
-constexpr int kPfTile = 128;                                    // KV tokens per tile
 constexpr int kPfHalfTileBytes = kPfTile * 128;                 // [128 tokens][64 dims] bf16
 constexpr int kPfTileBytes = 2 * kPfHalfTileBytes;              // K or V tile: 32 KB
-constexpr int kPfItemInts = 8;
-constexpr int kPfMagic = 0x70663030;
-
-struct PrefillItem {
-  int32_t seq, kv_head, row0, n_tiles;        // row0: first packed row of the pair this item owns
-  int32_t kv_len, q_start, q_len, causal_base;
-};
-static_assert(sizeof(PrefillItem) == kPfItemInts * 4, "item layout");
-
-// The order in which an item walks its KV tiles is free (online softmax), so every item
-// starts at a different tile and wraps around: the row tiles of one (sequence, kv head)
-// pair run on different SMs at the same time, and walking in step they would all ask the
-// L2 for the same lines at the same moment.
-constexpr int kPfTileRotation = 5;
-__device__ __forceinline__ int first_tile(const PrefillItem& item) {
-  return item.n_tiles > 0 ? ((item.row0 / kPfRows) * kPfTileRotation) % item.n_tiles : 0;
-}
 
 struct PrefillParams {
   const __nv_bfloat16* q;
@@ -113,11 +93,6 @@ constexpr int kTcThreads = kTcSoftmaxThreads + 128 + kTcEpilogueThreads;   // wh
 // registers per thread after the hand-over below: 256 * 200 + 128 * 40 + 128 * 72 = 512 * 128
 constexpr int kTcRegsSoftmax = 200;
 
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 constexpr int kTcRegsOther = 40;
 constexpr int kTcRegsEpilogue = 72;
 constexpr int kTcTmemCols = 512;          // S0 [0,128) S1 [128,256) O [256,384) P_A [384,448) P_B [448,512)

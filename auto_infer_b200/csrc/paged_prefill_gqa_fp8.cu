@@ -1,0 +1,836 @@
+// Paged GQA attention for wide query blocks over an 8-bit cache (chunked prefill, multi-token
+// verify): any q_len, bottom-right causal, on tcgen05 with accumulators in tensor memory.
+//
+//   o = sum_j softmax_j(scale * q . (ck_j s_k)) * (cv_j s_v)
+//
+// Work items, queue, warp roles and the two softmax groups over one O are those of the 16-bit kernel:
+// 128 packed query rows of a (sequence, kv head) pair per item, one persistent CTA per SM.  What
+// the 8-bit cache changes:
+//
+// * S = Q K^T runs as kind::f8f6f4 on the codes as TMA brings them, without converting K.  Q is split
+//   into two e4m3 terms, q = 2^-u (hi + lo) with a power of two per row that brings the row's largest
+//   magnitude to [2^7, 2^8): hi = e4m3(2^u q) leaves a rest of at most 4 significant bits of a
+//   bf16 q, which lo holds exactly (elements below 2^-10 of the row's largest: to 2^-18 of it).  Two
+//   K = 32 MMAs read the bytes that two K = 16 MMAs of the 16-bit kernel read, so S costs the same tensor
+//   and shared-memory time and K half of the loads.
+// * V is converted to f16 (exact) by the warpgroup that also writes O: splitting P like Q would cost the
+//   softmax threads, which set the pace, five instructions per pair of weights, while that warpgroup idles
+//   between items.  P is f16, three more bits than bf16.
+// * No element is multiplied by a scale.  K's scale and the row's 2^-u are in the factor that
+//   turns a product into a log2 score; V's scale is in the weight, w = 2^(x + log2 s_v - M) with M the running
+//   maximum of x + log2 s_v (handed between the groups with O), while each group's row sum refers to its own
+//   running maximum m of x.  A page is at least 16 tokens: a tile has 8 column groups of 16, each with its
+//   scales, or one pair for the whole tile when pages hold 128 tokens or more.
+//
+// Tensor-bound: flops = 4 * 128 * sum over rows of visible keys.
+#define B200_INLINE_WAITS
+#include "fp8.cuh"
+#include "prefill_plan.cuh"
+#include "tc05.cuh"
+
+namespace b200 {
+
+constexpr int kP8TileBytes = kPfTile * kFp8HeadDim;             // K or V codes of a tile: 16 KB
+constexpr int kP8KStages = 3;
+constexpr int kP8VStages = 2;                                   // codes; two more tiles wait as f16
+constexpr int kP8KLead = 2;                                     // K loads run this many tiles ahead of the V loads
+constexpr int kP8ScaleSlots = 8;
+constexpr int kP8Groups = kPfTile / kFp8MinBlockSize;           // column groups of a tile: 8
+constexpr int kP8SoftmaxThreads = 256;
+constexpr int kP8ConvertThreads = 128;
+constexpr int kP8Threads = kP8SoftmaxThreads + 128 + kP8ConvertThreads;   // whole warpgroups: 512 = 4 x 128
+// registers per thread after the hand-over: 256 * 200 + 128 * 40 + 128 * 72 = 512 * 128
+constexpr int kP8RegsSoftmax = 200;
+constexpr int kP8RegsOther = 40;
+constexpr int kP8RegsConvert = 72;
+constexpr int kP8TmemCols = 512;          // S0 [0,128) S1 [128,256) O [256,384) P_A [384,448) P_B [448,512)
+constexpr int kP8OCol = 256;
+constexpr int kP8PCol = 384;
+
+struct __align__(1024) Prefill8Smem {
+  uint8_t q[2][2][kPfRows * kFp8HeadDim];  // per item parity: hi, lo; [128 rows][128 B], swizzled
+  uint8_t k[kP8KStages][kP8TileBytes];     // [128 tokens][128 B], swizzled
+  uint8_t v[kP8VStages][kP8TileBytes];
+  uint8_t v16[2][2 * kP8TileBytes];        // f16: [dims 0-63 | dims 64-127], 128 tokens x 128 B each, swizzled
+  float row_factor[2][kPfRows];            // per item parity: softmax scale * log2(e) * 2^-u of the row
+  float row_l[2][kPfRows];                 // end of item: the groups' row sums
+  float row_m[2][kPfRows];                 // and the maxima they refer to
+  float row_mfin[kPfRows];                 // end of item: the reference of O
+  float row_ms[2][kPfRows];                // running reference of O after tile j, slot j & 1
+  float tile_scale[kP8ScaleSlots][2][kP8Groups];   // K, V scales of a tile's column groups
+  uint64_t k_full[kP8KStages];
+  uint64_t k_empty[kP8KStages];
+  uint64_t v_full[kP8VStages];
+  uint64_t v_empty[kP8VStages];
+  uint64_t v16_full[2];                    // freed by pv_done
+  uint64_t scale_full[kP8ScaleSlots];      // a slot is reused 8 tiles on, when its readers are long through
+  uint64_t s_full[2];
+  uint64_t s_empty[2];                     // softmax threads: the tile's scores and scales are in registers
+  uint64_t p_full[2];                      // per group
+  uint64_t pv_done[2];                     // per tile parity
+  uint64_t m_ready[2];                     // per tile parity: row_ms[parity] is written
+  uint64_t o_done;                         // P V issuer -> convert warps: the item's O is complete
+  uint64_t o_free;                         // convert warps -> P V issuer: O is in registers
+  uint64_t l_full;                         // softmax threads -> convert warps: row_l / row_m / row_mfin written
+  uint64_t l_empty;                        // and read
+  uint64_t q_full[2];                      // per item parity: the Q terms and row factors are staged
+  uint64_t q_empty[2];                     // all S MMAs of the item have run
+  uint64_t item_full[2];                   // work-queue hand-off: producer warp -> the other roles
+  uint64_t item_empty[2];
+  alignas(16) PrefillItem next_rec[2];     // the mailbox carries the whole item record (read as int4)
+  int next_item[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Prefill8Smem) <= 227 * 1024, "shared memory budget of one CTA");
+
+struct Prefill8Params {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  const float* scale_of[2];         // (num_blocks, Hkv), K and V
+  const int32_t* block_table;
+  int64_t bt_stride;
+  int table_rows, table_cols;
+  int num_tokens;
+  const PrefillItem* items;
+  int* work_counter;                // two plan words: next item to hand out, CTAs that have left
+                                    // (the word before them is the number of items)
+  void* out;
+  float* lse_out;
+  int32_t* status;
+  int num_q_heads, num_kv_heads, group;
+  int block_size, block_shift, num_blocks, box_tokens, boxes_per_tile;
+  int out_is_f32;
+  float scale_log2;
+};
+
+// Instruction descriptor with fp32 accumulation and operand type 0: f16 in kind::f16, e4m3 in kind::f8f6f4.
+__host__ __device__ constexpr uint32_t umma_idesc_type0(int m, int n, bool b_mn_major) {
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// D[tmem] (+)= A[smem] * B[smem] on 8-bit codes, K = 32.
+template <bool kAccumulate>
+__device__ __forceinline__ void umma_f8_ss_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                              uint32_t b_hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .b64 da, db;\n\t.reg .pred p;\n\t"
+      "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+      "setp.ne.u32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t}"
+      ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(kAccumulate ? 1 : 0));
+}
+template <bool kOnePage>   // pages of 128 tokens or more: one pair of scales per tile
+__global__ void __launch_bounds__(kP8Threads, 1)
+paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                         const Prefill8Params p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Prefill8Smem& sm = *reinterpret_cast<Prefill8Smem*>(smem_raw);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (smem_u32(smem_raw) & 1023u) {       // the swizzled tiles need a 1024-byte aligned base
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    sm.abort_flag = 0;
+    for (int s = 0; s < kP8KStages; ++s) {
+      mbar_init(&sm.k_full[s], 1);
+      mbar_init(&sm.k_empty[s], 1);
+    }
+    for (int s = 0; s < kP8VStages; ++s) {
+      mbar_init(&sm.v_full[s], 1);
+      mbar_init(&sm.v_empty[s], kP8ConvertThreads);
+    }
+    for (int s = 0; s < kP8ScaleSlots; ++s) mbar_init(&sm.scale_full[s], 32);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.v16_full[b], kP8ConvertThreads);
+      mbar_init(&sm.s_full[b], 1);
+      mbar_init(&sm.s_empty[b], 128);
+      mbar_init(&sm.p_full[b], 128);
+      mbar_init(&sm.pv_done[b], 1);
+      mbar_init(&sm.m_ready[b], 128);
+      mbar_init(&sm.q_full[b], kP8ConvertThreads);
+      mbar_init(&sm.q_empty[b], 1);
+      mbar_init(&sm.item_full[b], 1);
+      mbar_init(&sm.item_empty[b], kP8SoftmaxThreads + 2 + kP8ConvertThreads);   // all consumers of the mailbox
+    }
+    mbar_init(&sm.o_done, 1);
+    mbar_init(&sm.o_free, kP8ConvertThreads);
+    mbar_init(&sm.l_full, kP8SoftmaxThreads);
+    mbar_init(&sm.l_empty, kP8ConvertThreads);
+    mbar_fence_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&sm.tmem_base, kP8TmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dep_wait();                // q and the step's new cache rows come from earlier kernels
+  const uint32_t tmem = sm.tmem_base;
+  volatile int* abort_flag = &sm.abort_flag;
+  // Items are handed out dynamically, longest first: the producer warp draws the next index from a
+  // global counter and passes it to the other roles through a two-slot mailbox.  -1 ends the CTA.
+  auto take_item = [&](uint32_t k, PrefillItem& rec) -> int {
+    mbar_wait_bounded(&sm.item_full[k & 1u], (k >> 1) & 1u, abort_flag, p.status);
+    const int idx = *reinterpret_cast<volatile int*>(&sm.next_item[k & 1u]);
+    const int4* src = reinterpret_cast<const int4*>(&sm.next_rec[k & 1u]);
+    const int4 lo = src[0], hi = src[1];
+    rec = PrefillItem{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    mbar_arrive(&sm.item_empty[k & 1u]);
+    return (*abort_flag || idx < 0) ? -1 : idx;
+  };
+
+  if (warp >= 8 && warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kP8RegsOther));
+    if (warp == 8) {
+      // ------------------------------ TMA producer ------------------------------
+      if (lane == 0) {
+        tma_prefetch_desc(&k_map);
+        tma_prefetch_desc(&v_map);
+      }
+      uint32_t it = 0;
+      const int nbox = p.boxes_per_tile;
+      auto draw = [&](uint32_t k) -> int {
+        int idx = -1;
+        if (lane == 0) {
+          // the first item of a CTA is its own index; the rest of the list is handed out dynamically
+          idx = (k == 0) ? (int)blockIdx.x : (int)gridDim.x + atomicAdd(p.work_counter, 1);
+          if (idx >= __ldg(p.work_counter - 1) || *abort_flag) idx = -1;
+          mbar_wait_bounded(&sm.item_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_flag, p.status);
+          if (idx >= 0) {
+            const int4* src = reinterpret_cast<const int4*>(p.items + idx);
+            int4* dst = reinterpret_cast<int4*>(&sm.next_rec[k & 1u]);
+            dst[0] = __ldg(src);
+            dst[1] = __ldg(src + 1);
+          }
+          sm.next_item[k & 1u] = idx;
+          mbar_arrive(&sm.item_full[k & 1u]);     // release semantics: index and record are visible to waiters
+        }
+        idx = __shfl_sync(0xffffffffu, idx, 0);
+        return idx;
+      };
+      int idx = draw(0);
+      for (uint32_t k = 0; idx >= 0; ++k) {
+        const PrefillItem item = sm.next_rec[k & 1u];   // not overwritten before this warp draws item k + 2
+        const int last_block = (item.kv_len - 1) >> p.block_shift;
+        const int rot = first_tile(item);
+        // Lane g < 8 looks up the page of the tile's column group g; a box is box_tokens / 16 groups.
+        // K and V travel through separate rings (a K stage is free again as soon as S = Q K^T has run), the K
+        // loads kP8KLead tiles ahead of the V loads.
+        auto issue = [&](bool is_k, int step, uint32_t itx) {
+          int tile = step + rot;
+          if (tile >= item.n_tiles) tile -= item.n_tiles;
+          int bid = -1;
+          if (lane < kP8Groups) {
+            int lb = (tile * kPfTile + lane * kFp8MinBlockSize) >> p.block_shift;
+            lb = lb > last_block ? last_block : lb;                  // the tail re-reads the last valid page
+            if (item.seq < p.table_rows && lb < p.table_cols)
+              bid = p.block_table[(int64_t)item.seq * p.bt_stride + lb];
+            if (bid >= p.num_blocks) bid = -1;
+            if (bid < 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_BLOCK);
+          }
+          const int box_bid = __shfl_sync(0xffffffffu, bid, (lane * (p.box_tokens / kFp8MinBlockSize)) & 31);
+          const int tok = (tile * kPfTile + lane * p.box_tokens) & (p.block_size - 1);
+          const int b = box_bid < 0 ? p.num_blocks : box_bid;        // outside: TMA fills zeros
+          if (is_k) {
+            const int sk = itx % kP8KStages;
+            if (lane == 0) {
+              mbar_wait_bounded(&sm.k_empty[sk], ((itx / kP8KStages) & 1u) ^ 1u, abort_flag, p.status);
+              mbar_arrive_expect_tx(&sm.k_full[sk], kP8TileBytes);
+            }
+            __syncwarp();
+            if (lane < nbox)
+              tma_load_4d(sm.k[sk] + lane * p.box_tokens * kFp8HeadDim, &k_map, &sm.k_full[sk], 0, item.kv_head, tok, b);
+            // The tile's scales, through a ring of their own: the K stage is handed back before the softmax
+            // threads read them.  Slot itx - 8 is free: the K stage this tile takes was freed by S of tile
+            // itx - 3, whose score buffer was handed back by the readers of tile itx - 5.
+            const uint32_t sl = itx % kP8ScaleSlots;
+            if (lane < kP8Groups) {
+              const int64_t at = bid < 0 ? 0 : (int64_t)bid * p.num_kv_heads + item.kv_head;
+              cp_async_f32(&sm.tile_scale[sl][0][lane], p.scale_of[0] + at, bid >= 0);
+              cp_async_f32(&sm.tile_scale[sl][1][lane], p.scale_of[1] + at, bid >= 0);
+            }
+            cp_async_arrive(&sm.scale_full[sl]);
+          } else {
+            const int sv = itx % kP8VStages;
+            if (lane == 0) {
+              mbar_wait_bounded(&sm.v_empty[sv], ((itx / kP8VStages) & 1u) ^ 1u, abort_flag, p.status);
+              mbar_arrive_expect_tx(&sm.v_full[sv], kP8TileBytes);
+            }
+            __syncwarp();
+            if (lane < nbox)
+              tma_load_4d(sm.v[sv] + lane * p.box_tokens * kFp8HeadDim, &v_map, &sm.v_full[sv], 0, item.kv_head, tok, b);
+          }
+          __syncwarp();
+        };
+        // The next item is drawn four tiles before this one's last load: the convert warps stage its Q
+        // while this item's last tiles are worked on.
+        int next = -1;
+        const int draw_at = item.n_tiles > 4 ? item.n_tiles - 4 : 0;
+        int kt = 0;                                  // next K tile to request
+        for (int tile = 0; tile < item.n_tiles; ++tile) {
+          if (tile == draw_at) next = draw(k + 1);
+          for (; kt < item.n_tiles && kt <= tile + kP8KLead; ++kt) issue(true, kt, it + kt);
+          issue(false, tile, it + tile);
+        }
+        if (item.n_tiles == 0) next = draw(k + 1);
+        it += item.n_tiles;
+        idx = next;
+      }
+      // drain: nothing may still be landing when the CTA leaves
+      if (lane == 0) {
+        for (uint32_t k = 0; k < (uint32_t)kP8KStages && k < it; ++k) {
+          const uint32_t j = it - 1 - k;
+          mbar_wait_bounded(&sm.k_full[j % kP8KStages], (j / kP8KStages) & 1u, abort_flag, p.status);
+        }
+        for (uint32_t k = 0; k < (uint32_t)kP8VStages && k < it; ++k) {
+          const uint32_t j = it - 1 - k;
+          mbar_wait_bounded(&sm.v_full[j % kP8VStages], (j / kP8VStages) & 1u, abort_flag, p.status);
+        }
+        for (uint32_t k = 0; k < (uint32_t)kP8ScaleSlots && k < it; ++k) {
+          const uint32_t j = it - 1 - k;
+          mbar_wait_bounded(&sm.scale_full[j % kP8ScaleSlots], (j / kP8ScaleSlots) & 1u, abort_flag, p.status);
+        }
+      }
+    } else if (warp == 9) {
+      // ------------------------- MMA issuer: S = Q K^T -------------------------
+      if (lane == 0) {
+        constexpr uint32_t idesc = umma_idesc_type0(kPfRows, kPfTile, false);
+        // descriptors differ only in their start-address field: build once, add offsets
+        const uint64_t dq = umma_desc_sw128(smem_u32(sm.q[0][0]), 16, 1024);
+        const uint64_t dk = umma_desc_sw128(smem_u32(sm.k[0]), 16, 1024);
+        const uint32_t dq_lo = (uint32_t)dq, dq_hi = (uint32_t)(dq >> 32);
+        const uint32_t dk_lo = (uint32_t)dk, dk_hi = (uint32_t)(dk >> 32);
+        constexpr uint32_t kTerm = (kPfRows * kFp8HeadDim) >> 4;   // one Q term, in descriptor units
+        uint32_t it = 0;
+        for (uint32_t item_no = 0;; ++item_no) {
+          PrefillItem rec;
+          if (take_item(item_no, rec) < 0) break;
+          const int n_tiles = rec.n_tiles;
+          const uint32_t qb = item_no & 1u;
+          mbar_wait_bounded(&sm.q_full[qb], (item_no >> 1) & 1u, abort_flag, p.status);
+          const uint32_t q_lo = dq_lo + qb * 2 * kTerm;
+          if (n_tiles == 0) umma_commit(&sm.q_empty[qb]);
+          for (int tile = 0; tile < n_tiles; ++tile, ++it) {
+            const int s = it % kP8KStages;
+            const int b = it & 1u;
+            mbar_wait_bounded(&sm.k_full[s], (it / kP8KStages) & 1u, abort_flag, p.status);
+            mbar_wait_bounded(&sm.s_empty[b], ((it >> 1) & 1u) ^ 1u, abort_flag, p.status);
+            tc_fence_after();
+            const uint32_t k_lo = dk_lo + (uint32_t)((s * kP8TileBytes) >> 4);
+            const uint32_t d_tmem = tmem + b * 128;
+            umma_f8_ss_lo<false>(d_tmem, q_lo, dq_hi, k_lo, dk_hi, idesc);
+#pragma unroll
+            for (int i = 1; i < 8; ++i)             // four K = 32 steps of hi, four of lo
+              umma_f8_ss_lo<true>(d_tmem, q_lo + (i >> 2) * kTerm + (i & 3) * 2, dq_hi, k_lo + (i & 3) * 2, dk_hi, idesc);
+            umma_commit(&sm.s_full[b]);
+            umma_commit(&sm.k_empty[s]);
+            if (tile == n_tiles - 1) umma_commit(&sm.q_empty[qb]);   // the Q terms may be overwritten
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == 10) {
+      // ------------------------- MMA issuer: O += P V --------------------------
+      if (lane == 0) {
+        constexpr uint32_t idesc = umma_idesc_type0(kPfRows, kPfHeadDim, true);
+        const uint64_t dv = umma_desc_sw128(smem_u32(sm.v16[0]), kP8TileBytes, 1024);
+        const uint32_t dv_lo = (uint32_t)dv, dv_hi = (uint32_t)(dv >> 32);
+        uint32_t it = 0;
+        for (uint32_t item_no = 0;; ++item_no) {
+          PrefillItem rec;
+          if (take_item(item_no, rec) < 0) break;
+          const int n_tiles = rec.n_tiles;
+          for (int tile = 0; tile < n_tiles; ++tile, ++it) {
+            const int g = it & 1u;                            // the group that owns this tile, and its V buffer
+            mbar_wait_bounded(&sm.v16_full[g], (it >> 1) & 1u, abort_flag, p.status);
+            mbar_wait_bounded(&sm.p_full[g], (it >> 1) & 1u, abort_flag, p.status);
+            if (tile == 0 && item_no > 0)                     // the previous item's O has been read
+              mbar_wait_bounded(&sm.o_free, (item_no - 1) & 1u, abort_flag, p.status);
+            tc_fence_after();
+            const uint32_t v_lo = dv_lo + (uint32_t)((g * 2 * kP8TileBytes) >> 4);
+            const uint32_t p_tmem = tmem + kP8PCol + g * 64;  // P of the tile: 128 tokens as f16 pairs
+            const uint32_t d_tmem = tmem + kP8OCol;
+            if (tile == 0)                                    // the first tile of the item overwrites
+              umma_bf16_ts_lo<false>(d_tmem, p_tmem, v_lo, dv_hi, idesc);
+            else
+              umma_bf16_ts_lo<true>(d_tmem, p_tmem, v_lo, dv_hi, idesc);
+#pragma unroll
+            for (int ks = 1; ks < kPfTile / 16; ++ks)
+              umma_bf16_ts_lo<true>(d_tmem, p_tmem + ks * 8, v_lo + (uint32_t)((ks * 2048) >> 4), dv_hi, idesc);
+            umma_commit(&sm.pv_done[g]);
+          }
+          umma_commit(&sm.o_done);
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kP8RegsSoftmax));
+    // -------------------------------- softmax --------------------------------
+    const int g = warp >> 2;                         // group: KV tiles whose running index & 1 == g
+    const int r = threadIdx.x & 127;                 // query row of the tile == TMEM lane
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t o_col = lane_base + kP8OCol;
+    const uint32_t p_col = lane_base + kP8PCol + g * 64;
+    const int G = p.group;
+    uint32_t it = 0;
+    for (uint32_t item_no = 0;; ++item_no) {
+      PrefillItem item;
+      if (take_item(item_no, item) < 0) break;
+      const int rg = item.row0 + r;
+      const bool valid = rg < item.q_len * G;
+      const int lim = valid ? min(item.causal_base + rg / G, item.kv_len - 1) : -1;
+      const int rot = first_tile(item);
+      mbar_wait_bounded(&sm.q_full[item_no & 1u], (item_no >> 1) & 1u, abort_flag, p.status);
+      const float row_factor = sm.row_factor[item_no & 1u][r];
+      float m = -INFINITY;           // running maximum of this group's scores: what its row sum is scaled to
+      float l = 0.f;
+      for (int tile = 0; tile < item.n_tiles; ++tile, ++it) {
+        if ((int)(it & 1u) != g) continue;             // the other group's tile
+        const uint32_t sb = it & 1u;
+        const uint32_t s_col = lane_base + sb * 128;
+        constexpr int kN = kOnePage ? 1 : kP8Groups;   // pairs of scales of a tile
+        const uint32_t sl = it % kP8ScaleSlots;
+        mbar_wait_bounded(&sm.scale_full[sl], (it / kP8ScaleSlots) & 1u, abort_flag, p.status);
+        float f[kN], lv[kN];                           // product -> log2 score; log2 of V's scale
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          f[i] = row_factor * sm.tile_scale[sl][0][i];
+          // not 0, which would make NaN of the -inf that masks (a NaN scale stays NaN)
+          f[i] = f[i] < 1.17549435e-38f ? 1.17549435e-38f : f[i];
+          lv[i] = fast_log2(sm.tile_scale[sl][1][i]);
+        }
+        mbar_wait_bounded(&sm.s_full[sb], (it >> 1) & 1u, abort_flag, p.status);
+        tc_fence_after();
+        int kv_tile = tile + rot;                      // the KV tile this step works on
+        if (kv_tile >= item.n_tiles) kv_tile -= item.n_tiles;
+        const int tbase = kv_tile * kPfTile;
+        const bool need_mask = tbase + kPfTile - 1 > lim;
+        // The whole score row goes to registers in one go and the S buffer straight back to
+        // the MMA issuer.
+        uint32_t sv[4][32];
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) tmem_ld32(s_col + q4 * 32, sv[q4]);
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(&sm.s_empty[sb]);
+        if (need_mask) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (tbase + q4 * 32 + c > lim) sv[q4][c] = __float_as_uint(-INFINITY);
+        }
+        // maximum of the scores, and of the scores plus log2 of V's scale
+        float mx = -INFINITY, my = -INFINITY;
+        {
+          float mq[8];                      // one chain per column group
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            mq[u] = fmaxf(__uint_as_float(sv[u >> 1][(u & 1) * 16]), __uint_as_float(sv[u >> 1][(u & 1) * 16 + 1]));
+#pragma unroll
+          for (int c = 2; c < 16; c += 2)
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              mq[u] = fmax3(mq[u], __uint_as_float(sv[u >> 1][(u & 1) * 16 + c]),
+                            __uint_as_float(sv[u >> 1][(u & 1) * 16 + c + 1]));
+          if constexpr (kOnePage) {
+            mx = fmaxf(fmax3(mq[0], mq[1], mq[2]), fmax3(fmax3(mq[3], mq[4], mq[5]), mq[6], mq[7])) * f[0];
+            my = mx + lv[0];
+          } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const float x = mq[u] * f[u];
+              mx = fmaxf(mx, x);
+              my = fmaxf(my, x + lv[u]);
+            }
+          }
+        }
+        // the reference O is scaled to after the previous tile (owned by the other group)
+        float m_in = -INFINITY;
+        if (tile > 0) {
+          mbar_wait_bounded(&sm.m_ready[(it - 1) & 1u], ((it - 1) >> 1) & 1u, abort_flag, p.status);
+          m_in = sm.row_ms[(it - 1) & 1u][r];
+        }
+        // lazy rescale: only when some row of the warp outgrew the stale reference by 2^8
+        const bool grow = my - m_in > 8.f || (m_in == -INFINITY && my > -INFINITY);
+        const bool rescale = __any_sync(0xffffffffu, grow);
+        const float m_used = rescale ? fmaxf(m_in, my) : m_in;
+        sm.row_ms[it & 1u][r] = m_used;
+        mbar_arrive(&sm.m_ready[it & 1u]);             // release: the next tile's owner may go on
+        const float m_new = fmaxf(m, mx);
+        const float m_sub = m_new == -INFINITY ? 0.f : m_new;
+        l *= fast_exp2(m - m_sub);                     // m = -inf: l is 0
+        m = m_new;
+        const float o_sub = m_used == -INFINITY ? 0.f : m_used;
+        // w = 2^(x + lv - o_sub) = p 2^e with p = 2^(x - m) and e uniform over a column group; the row sum
+        // takes 2^-e sum w.  Below 2^-60 a weight is 0 in f16 whatever it is: e stops there so that p
+        // itself is not lost from the sum.
+        float shift[kN], undo[kN];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          float e = m_sub + lv[i] - o_sub;
+          e = e < -60.f ? -60.f : e > 120.f ? 120.f : e;
+          shift[i] = e - m_sub;
+          undo[i] = fast_exp2(-e);
+        }
+        // The group's P buffer is free once the P V of its previous tile (of this item or the
+        // one before) has run.  The group waited for the one before that two tiles ago, so
+        // the parity wait cannot be off by a phase.
+        if (it >= 2) {
+          mbar_wait_bounded(&sm.pv_done[g], ((it - 2) >> 1) & 1u, abort_flag, p.status);
+          tc_fence_after();
+        }
+        // O may be touched once the previous tile's P V (the other group's) has run: rare path
+        if (rescale && tile > 0) {
+          const float corr = (m_in == -INFINITY) ? 0.f : fast_exp2(m_in - m_used);
+          mbar_wait_bounded(&sm.pv_done[g ^ 1], ((it - 1) >> 1) & 1u, abort_flag, p.status);
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t orow[32];
+            tmem_ld32(o_col + c * 32, orow);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) orow[i] = __float_as_uint(__uint_as_float(orow[i]) * corr);
+            tmem_st32(o_col + c * 32, orow);
+          }
+        }
+        // Weights, software-pipelined by a quarter of the row: the exponentials of quarter q are issued while
+        // quarter q - 1 is summed and packed.  P (f16 pairs) goes to the group's buffer 64 columns at a time.
+        float2 ls[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+        uint32_t pk[32];
+#pragma unroll
+        for (int q4 = 0; q4 <= 4; ++q4) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            if (q4 < 4) {
+              const int u = kOnePage ? 0 : q4 * 2 + (c >> 4);
+              const float2 x = __ffma2_rn(make_float2(__uint_as_float(sv[q4][c]), __uint_as_float(sv[q4][c + 1])),
+                                          make_float2(f[u], f[u]), make_float2(shift[u], shift[u]));
+              sv[q4][c] = __float_as_uint(fast_exp2(x.x));
+              sv[q4][c + 1] = __float_as_uint(fast_exp2(x.y));
+            }
+            if (q4 > 0) {
+              const float2 pp = make_float2(__uint_as_float(sv[q4 - 1][c]), __uint_as_float(sv[q4 - 1][c + 1]));
+              if constexpr (kOnePage) {
+                ls[(c >> 1) & 3] = __fadd2_rn(ls[(c >> 1) & 3], pp);
+              } else {
+                const int u = (q4 - 1) * 2 + (c >> 4);
+                ls[(c >> 1) & 3] = __ffma2_rn(pp, make_float2(undo[u], undo[u]), ls[(c >> 1) & 3]);
+              }
+              pk[((q4 - 1) & 1) * 16 + (c >> 1)] = pack_f16(pp.x, pp.y);
+            }
+          }
+          if (q4 == 2) tmem_st32(p_col, pk);
+          if (q4 == 4) tmem_st32(p_col + 32, pk);
+        }
+        {
+          const float2 a = __fadd2_rn(ls[0], ls[1]), b = __fadd2_rn(ls[2], ls[3]);
+          const float sum = (a.x + a.y) + (b.x + b.y);
+          l += kOnePage ? sum * undo[0] : sum;
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sm.p_full[g]);
+      }
+      // ---- hand the row sums to the convert warps and go on with the next item
+      // the references only grow along the tiles: the last tile's is what O is scaled to
+      float mm = -INFINITY;
+      if (item.n_tiles > 0) {
+        mbar_wait_bounded(&sm.m_ready[(it - 1) & 1u], ((it - 1) >> 1) & 1u, abort_flag, p.status);
+        mm = sm.row_ms[(it - 1) & 1u][r];
+      }
+      if (item_no > 0) mbar_wait_bounded(&sm.l_empty, (item_no - 1) & 1u, abort_flag, p.status);
+      sm.row_l[g][r] = l;
+      sm.row_m[g][r] = m;
+      if (g == 0) sm.row_mfin[r] = mm;
+      mbar_arrive(&sm.l_full);
+    }
+  } else {
+    // ------------------- convert: Q terms, V to f16, epilogue -------------------
+    // Thread e owns query row e: it stages the row's two e4m3 terms two tiles before the previous
+    // item ends, and takes row e of O out of tensor memory at the end.  In between the 128 threads turn
+    // each V tile's codes into f16, one tile ahead of its P V or more.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kP8RegsConvert));
+    const int r = threadIdx.x - (kP8Threads - kP8ConvertThreads);
+    const uint32_t o_col = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kP8OCol;
+    const int G = p.group;
+    uint32_t it = 0;                                 // next V tile to convert, over all items
+    auto rows_of = [&](const PrefillItem& x) -> int {
+      return x.q_start + x.q_len <= p.num_tokens ? x.q_len * G : 0;
+    };
+    auto stage_q = [&](const PrefillItem& x, uint32_t k) {
+      const int rg = x.row0 + r;
+      const bool valid = rg < rows_of(x);
+      if (r == 0 && rows_of(x) < x.q_len * G && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(valid ? x.q_start + rg / G : 0) * p.q_stride +
+                                                        (int64_t)(valid ? x.kv_head * G + rg % G : 0) * kPfHeadDim);
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int c0 = 0; c0 < 16; c0 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = valid ? src[c0 + c] : zero;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+        }
+      }
+      const int e = max((int)(top >> 7), 8);                       // exponent field; 8 and more: both factors are normal
+      const float up = __uint_as_float((uint32_t)(261 - e) << 23); // 2^(7 - (e - 127))
+      mbar_wait_bounded(&sm.q_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_flag, p.status);
+      uint8_t* const hi_at = sm.q[k & 1u][0];
+      uint8_t* const lo_at = sm.q[k & 1u][1];
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {                                // 16 dims at a time
+        const uint4 a = valid ? src[2 * c] : zero, b = valid ? src[2 * c + 1] : zero;
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            x[2 * j] = __uint_as_float(w[2 * i + j] << 16) * up;
+            x[2 * j + 1] = __uint_as_float(w[2 * i + j] & 0xffff0000u) * up;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = fmaf(x[j], 0.f, x[j]);  // infinities become NaN, which has a code
+          hi[i] = f32x4_to_e4m3x4(x[0], x[1], x[2], x[3]);
+          const uint32_t h0 = e4m3x2_to_f16x2((uint16_t)hi[i]), h1 = e4m3x2_to_f16x2((uint16_t)(hi[i] >> 16));
+          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+          const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+          lo[i] = f32x4_to_e4m3x4(x[0] - f0.x, x[1] - f0.y, x[2] - f1.x, x[3] - f1.y);
+        }
+        *reinterpret_cast<uint4*>(hi_at + swz128(r, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(lo_at + swz128(r, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      sm.row_factor[k & 1u][r] = __uint_as_float((uint32_t)(e - 7) << 23) * p.scale_log2;
+      fence_proxy_async_smem();
+      mbar_arrive(&sm.q_full[k & 1u]);
+    };
+    // A thread takes the 16-byte chunk c of every 16th row: eight lanes read one row, all banks.  The 16
+    // codes become two chunks of f16, c >> 2 picks the half; lanes of the second half store their odd chunk
+    // first, so that the eight lanes of a phase again cover all banks.
+    const int c = r & 7;
+    auto convert = [&](const PrefillItem& x, int step) {
+      int kv_tile = step + first_tile(x);
+      if (kv_tile >= x.n_tiles) kv_tile -= x.n_tiles;
+      const int have = x.kv_len - kv_tile * kPfTile;               // rows past the end are zero: 0 x NaN is NaN
+      const int sv = it % kP8VStages, b = it & 1u;
+      mbar_wait_bounded(&sm.v_full[sv], (it / kP8VStages) & 1u, abort_flag, p.status);
+      if (it >= 2) mbar_wait_bounded(&sm.pv_done[b], ((it - 2) >> 1) & 1u, abort_flag, p.status);
+      const uint8_t* src = sm.v[sv];
+      uint8_t* dst = sm.v16[b] + (c >> 2) * kP8TileBytes;
+      const int first = 2 * (c & 3) + (c >> 2), second = 2 * (c & 3) + (1 - (c >> 2));
+#pragma unroll
+      for (int i0 = 0; i0 < 8; i0 += 4) {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = (r >> 3) + 16 * (i0 + i);
+          v[i] = *reinterpret_cast<const uint4*>(src + swz128(row, c));
+          if (row >= have) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = (r >> 3) + 16 * (i0 + i);
+          const uint4 lo = make_uint4(e4m3x2_to_f16x2((uint16_t)v[i].x), e4m3x2_to_f16x2((uint16_t)(v[i].x >> 16)),
+                                      e4m3x2_to_f16x2((uint16_t)v[i].y), e4m3x2_to_f16x2((uint16_t)(v[i].y >> 16)));
+          const uint4 hi = make_uint4(e4m3x2_to_f16x2((uint16_t)v[i].z), e4m3x2_to_f16x2((uint16_t)(v[i].z >> 16)),
+                                      e4m3x2_to_f16x2((uint16_t)v[i].w), e4m3x2_to_f16x2((uint16_t)(v[i].w >> 16)));
+          const bool odd_first = c >> 2;
+          *reinterpret_cast<uint4*>(dst + swz128(row, first)) = odd_first ? hi : lo;
+          *reinterpret_cast<uint4*>(dst + swz128(row, second)) = odd_first ? lo : hi;
+        }
+      }
+      mbar_arrive(&sm.v_empty[sv]);
+      fence_proxy_async_smem();
+      mbar_arrive(&sm.v16_full[b]);
+      ++it;
+    };
+    PrefillItem item, next;
+    int idx = take_item(0, item);
+    if (idx >= 0) {
+      stage_q(item, 0);
+      if (item.n_tiles > 0) convert(item, 0);
+    }
+    for (uint32_t item_no = 0; idx >= 0; ++item_no) {
+      // the next item's Q is staged before this item's last V tile, its first V tile right after
+      int next_idx = -1;
+      for (int tile = 1; tile < item.n_tiles; ++tile) {
+        if (tile == item.n_tiles - 1) {
+          next_idx = take_item(item_no + 1, next);
+          if (next_idx >= 0) stage_q(next, item_no + 1);
+        }
+        convert(item, tile);
+      }
+      if (item.n_tiles < 2) {
+        next_idx = take_item(item_no + 1, next);
+        if (next_idx >= 0) stage_q(next, item_no + 1);
+      }
+      if (next_idx >= 0 && next.n_tiles > 0) convert(next, 0);
+      // ---- epilogue: row e of O out of tensor memory as soon as the item's last P V has run
+      const int rg = item.row0 + r;
+      const bool valid = rg < rows_of(item);
+      const int64_t tok = item.q_start + (valid ? rg / G : 0);
+      const int head = item.kv_head * G + (valid ? rg % G : 0);
+      mbar_wait_bounded(&sm.l_full, item_no & 1u, abort_flag, p.status);
+      const float m0 = sm.row_m[0][r], m1 = sm.row_m[1][r], mo = sm.row_mfin[r];
+      const float mm = fmaxf(m0, m1);
+      // Which group had the item's even tiles depends on what the CTA worked on before: the two products
+      // are rounded alike (no fused multiply-add), so that the sum does not.
+      const float lsum = mm == -INFINITY ? sm.row_l[0][r] + sm.row_l[1][r]
+                                         : __fadd_rn(__fmul_rn(sm.row_l[0][r], fast_exp2(m0 - mm)),
+                                                     __fmul_rn(sm.row_l[1][r], fast_exp2(m1 - mm)));
+      mbar_arrive(&sm.l_empty);
+      // O is in units of 2^mo, the sum in units of 2^mm; the factor between them in two halves, each of
+      // which fp32 holds however far apart they are
+      const float half_unit = fast_exp2((mo - (mm == -INFINITY ? 0.f : mm)) * 0.5f);
+      const float inv = half_unit / lsum;
+      const bool empty = lsum == 0.f;      // no visible key: zeros, whatever the accumulator holds
+      mbar_wait_bounded(&sm.o_done, item_no & 1u, abort_flag, p.status);
+      tc_fence_after();
+#pragma unroll 1
+      for (int q4 = 0; q4 < 4; ++q4) {
+        uint32_t o[32];
+        tmem_ld32(o_col + q4 * 32, o);
+        tmem_wait_ld();
+        if (q4 == 3) {                       // the whole row is out of tensor memory
+          tc_fence_before();
+          mbar_arrive(&sm.o_free);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = empty ? 0u : __float_as_uint(__uint_as_float(o[i]) * half_unit * inv);
+        if (valid) {
+          const int64_t off = (tok * p.num_q_heads + head) * kPfHeadDim + q4 * 32;
+          if (p.out_is_f32) {
+            float* dst = reinterpret_cast<float*>(p.out) + off;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          } else {
+            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + off;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 v;
+              v.x = pack_bf16(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+              v.y = pack_bf16(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+              v.z = pack_bf16(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
+              v.w = pack_bf16(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
+              *reinterpret_cast<uint4*>(dst + i) = v;
+            }
+          }
+        }
+      }
+      if (valid && p.lse_out)
+        p.lse_out[tok * p.num_q_heads + head] = empty ? -INFINITY : mm * 0.6931471805599453f + __logf(lsum);
+      item = next;
+      idx = next_idx;
+    }
+  }
+  // ---- teardown: everyone is done with tensor memory before it is released
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kP8TmemCols);
+  }
+  // the last CTA to leave puts the queue back to zero for the next launch on this plan
+  if (threadIdx.x == 0) {
+    __threadfence();
+    if (atomicAdd(p.work_counter + 1, 1) == (int)gridDim.x - 1) {
+      p.work_counter[0] = 0;
+      p.work_counter[1] = 0;
+      __threadfence();
+    }
+  }
+}
+
+}  // namespace b200
+
+extern "C" int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride, const void* key_cache,
+                                          const void* value_cache, const float* key_scale,
+                                          const float* value_scale, int num_blocks, int block_size,
+                                          const int32_t* block_table, int64_t bt_stride, int table_rows,
+                                          int table_cols, int32_t* plan_dev, const b200_prefill_plan_info* info,
+                                          int max_ctas, int num_tokens, int num_q_heads, int num_kv_heads,
+                                          int head_dim, float scale, void* out, int out_is_f32, float* lse_out,
+                                          int32_t* status, void* stream) {
+  using namespace b200;
+  const char* who = "paged_prefill_gqa_fp8";
+  int rc = check_fp8_cache(who, key_cache, value_cache, key_scale, value_scale, num_blocks, block_size, num_kv_heads,
+                           head_dim);
+  if (rc) return rc;
+  if (info && info->num_items == 0) return B200_OK;
+  if (!q || !block_table || !plan_dev || !out || num_q_heads <= 0 || num_q_heads % num_kv_heads || num_tokens < 0 ||
+      max_ctas < 0 || table_rows <= 0 || table_cols <= 0) {
+    set_last_error("%s: null pointer, bad head counts, a negative size or an empty block table", who);
+    return B200_EINVAL;
+  }
+  if (reinterpret_cast<uintptr_t>(q) % 16 || q_stride % 8 || q_stride < (int64_t)num_q_heads * head_dim ||
+      reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(plan_dev) % 16) {
+    set_last_error("%s: q, out and the plan must be 16-byte aligned, the q token stride a multiple of 8 elements and >= Hq*D", who);
+    return B200_EALIGN;
+  }
+  const int box_tokens = block_size < kPfTile ? block_size : kPfTile;
+  CUtensorMap k_map, v_map;
+  rc = get_fp8_cache_tensor_map(key_cache, num_blocks, block_size, num_kv_heads, box_tokens, &k_map);
+  if (rc) return rc;
+  rc = get_fp8_cache_tensor_map(value_cache, num_blocks, block_size, num_kv_heads, box_tokens, &v_map);
+  if (rc) return rc;
+
+  Prefill8Params p;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride = q_stride;
+  p.scale_of[0] = key_scale;
+  p.scale_of[1] = value_scale;
+  p.block_table = block_table;
+  p.bt_stride = bt_stride;
+  p.table_rows = table_rows;
+  p.table_cols = table_cols;
+  p.num_tokens = num_tokens;
+  p.items = reinterpret_cast<const PrefillItem*>(plan_dev + kPlanHeaderInts);
+  p.work_counter = plan_dev + 2;
+  p.out = out;
+  p.lse_out = lse_out;
+  p.status = status;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads;
+  p.block_size = block_size;
+  p.block_shift = __builtin_ctz(block_size);
+  p.num_blocks = num_blocks;
+  p.box_tokens = box_tokens;
+  p.boxes_per_tile = kPfTile / box_tokens;
+  p.out_is_f32 = out_is_f32;
+  p.scale_log2 = scale * 1.4426950408889634f;
+
+  const bool one_page = block_size >= kPfTile;
+  auto kernel = one_page ? paged_prefill_fp8_kernel<true> : paged_prefill_fp8_kernel<false>;
+  const size_t smem = sizeof(Prefill8Smem);
+  static bool attr_set[2][64] = {{false}, {false}};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_set[one_page][dev]) {
+    rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                    "paged_prefill_gqa_fp8 smem attribute");
+    if (rc) return rc;
+    if (dev < 64) attr_set[one_page][dev] = true;
+  }
+  int grid = b200_sm_count();
+  if (grid <= 0) grid = 148;
+  if (info && grid > info->num_items) grid = info->num_items;
+  if (max_ctas > 0 && grid > max_ctas) grid = max_ctas;     // the rest of the SMs are left to another kernel
+  return check_cuda(launch_pdl(kernel, dim3(grid), dim3(kP8Threads), smem, static_cast<cudaStream_t>(stream), k_map,
+                               v_map, p),
+                    "paged_prefill_gqa_fp8 launch");
+}

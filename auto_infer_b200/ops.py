@@ -626,6 +626,29 @@ def paged_prefill_gqa(q: torch.Tensor, key_cache: torch.Tensor, value_cache: tor
     return out
 
 
+def paged_prefill_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                          key_scale: torch.Tensor, value_scale: torch.Tensor, block_table: torch.Tensor,
+                          plan: PrefillPlan, scale: float, out: Optional[torch.Tensor] = None,
+                          out_f32: bool = False, lse_out: Optional[torch.Tensor] = None,
+                          max_ctas: int = 0) -> torch.Tensor:
+    """``paged_prefill_gqa`` over an 8-bit cache (see ``reshape_and_cache_fp8``): the same plans, masks
+    and outputs.  Rows of sequences that are not in the plan are left untouched in ``out``."""
+    q, block_table, out, (num_blocks, block_size, n_kv, d) = _fp8_attention_args(
+        "paged_prefill_gqa_fp8", q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
+        lse_out)
+    with _on_device(q.device):
+        rc = _lib.load().b200_paged_prefill_gqa_fp8(
+            q.data_ptr(), q.stride(0), key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(),
+            value_scale.data_ptr(), num_blocks, block_size, block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[0], block_table.shape[1], plan.dev.data_ptr(),
+            None if plan.replayable else ctypes.byref(plan.info), int(max_ctas), q.shape[0], q.shape[1], n_kv, d,
+            float(scale), out.data_ptr(), 1 if out.dtype == torch.float32 else 0,
+            lse_out.data_ptr() if lse_out is not None else None,
+            status_word(q.device).data_ptr(), _stream_ptr(q.device))
+    _lib.check(rc, "b200_paged_prefill_gqa_fp8")
+    return out
+
+
 class MhaPlan:
     """Host plan + device copy + workspace of the K-192 / V-128 multi-head kernel (non-absorbed
     MLA): blocks of 64 query positions per head, keys cut into equal splits when the step has

@@ -345,6 +345,25 @@ int b200_paged_prefill_gqa_replayable(const void* q, int64_t q_stride,
                                       void* out, int out_is_f32, float* lse_out,
                                       int32_t* status, void* stream);
 
+/* The wide-query attention over an 8-bit cache (layout and scales as
+ * b200_reshape_and_cache_fp8).  Plans, masks, q, out and lse_out as
+ * b200_paged_prefill_gqa; max_ctas > 0 keeps it to that many SMs as _on does; with
+ * info == NULL the launch is the replayable one.  block_size, table_rows,
+ * table_cols, num_tokens and the scales as b200_paged_decode_gqa_fp8.  Cache rows
+ * past a sequence's kv_len may hold any codes; a NaN code of V in a row that one
+ * query row of a 128-row item sees makes NaN of that column for all rows of the item
+ * that share its 128-token tile, as a matrix product with a zero weight does. */
+int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride,
+                               const void* key_cache, const void* value_cache,
+                               const float* key_scale, const float* value_scale,
+                               int num_blocks, int block_size,
+                               const int32_t* block_table, int64_t bt_stride,
+                               int table_rows, int table_cols,
+                               int32_t* plan_dev, const b200_prefill_plan_info* info, int max_ctas,
+                               int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, float scale,
+                               void* out, int out_is_f32, float* lse_out,
+                               int32_t* status, void* stream);
+
 /* ------------------------------------------------------------------------ *
  * Same attention as b200_paged_decode_gqa for callers that may not allocate
  * device memory.  (No counterpart in the reference: its vendor op manages its

@@ -69,4 +69,37 @@ def attention(q, kc, vc, ks, vs, table, cu, kv_lens, scale, causal_base=None):
     return out, lse
 
 
-__all__ = ["E4M3", "as_values", "empty_pool", "random_pool", "deal_pages", "attention", "orc"]
+def smallest_weights(q, kc, vc, ks, vs, table, cu, kv_lens, scale, causal_base=None):
+    """2^-25 W sum_j |cv_j| per output element, W = max_j p_j s_v,j over the keys j a row sees.
+
+    What rounding the weights to f16 costs below f16's normal range.  A weight is taken relative to a
+    reference R <= W (the running maximum of p_j s_v,j, or one up to 2^8 below it), w_j = p_j s_v,j / R.  f16 is off
+    by at most half a step: 2^-11 w_j (half of 2^-10, and less) for w_j >= 2^-14, 2^-25 below.  The latter adds
+    at most 2^-25 R |cv_j| per key to a row's output, which is at most 2^-25 W sum_j |cv_j|.  It only shows where
+    the keys that carry the row have codes near 0 in a column."""
+    t, n_q, d = q.shape
+    bs, n_kv = kc.shape[1], kc.shape[2]
+    group = n_q // n_kv
+    out = torch.zeros(t, n_q, d, dtype=torch.float64)
+    q0 = 0
+    for b, end in enumerate(cu):
+        n, k_len = end - q0, kv_lens[b]
+        pages = table[b, :-(-k_len // bs)].long()
+        base = k_len - n if causal_base is None else causal_base[b]
+        for h in range(n_kv):
+            k = (as_values(kc[pages, :, h]) * ks[pages, h].double()[:, None, None]).reshape(-1, d)[:k_len]
+            codes = as_values(vc[pages, :, h]).reshape(-1, d)[:k_len].abs()
+            s_v = vs[pages, h].double().repeat_interleave(bs)[:k_len]
+            for i in range(n):
+                seen = max(0, min(base + i + 1, k_len))
+                if not seen:
+                    continue
+                heads = slice(h * group, (h + 1) * group)
+                p = torch.softmax(q[q0 + i, heads].double() @ k[:seen].T * scale, -1)
+                top = (p * s_v[:seen]).amax(-1, keepdim=True)
+                out[q0 + i, heads] = 2.0 ** -25 * top * codes[:seen].sum(0)
+        q0 = end
+    return out
+
+
+__all__ = ["smallest_weights", "E4M3", "as_values", "empty_pool", "random_pool", "deal_pages", "attention", "orc"]

@@ -84,3 +84,22 @@ def _decode_args(**change):
 def test_decode_refusals(lib, change, code):
     assert lib.b200_paged_decode_gqa_fp8(*_decode_args(**change)) == code
     assert b"paged_decode_gqa_fp8" in lib.b200_last_error()
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(q=None), -1), (dict(block_table=None), -1), (dict(plan=None), -1), (dict(out=None), -1), (dict(value_scale=None), -1),
+    (dict(num_q_heads=7), -1), (dict(num_tokens=-1), -1), (dict(max_ctas=-1), -1), (dict(table_cols=0), -1),
+    (dict(head_dim=256), -2), (dict(block_size=8), -2), (dict(q=(1 << 20) + 8), -3), (dict(q_stride=1028), -3),
+    (dict(out=(1 << 29) + 8), -3), (dict(plan=(1 << 27) + 4), -3),
+])
+def test_prefill_refusals(lib, change, code):
+    from auto_infer_b200._lib import PrefillPlanInfo
+    import ctypes
+    info = PrefillPlanInfo(num_items=1, num_tokens=1)
+    a = dict(q=1 << 20, q_stride=1024, key_cache=1 << 22, value_cache=1 << 23, key_scale=1 << 24, value_scale=1 << 25,
+             num_blocks=4, block_size=16, block_table=1 << 26, bt_stride=4, table_rows=1, table_cols=4, plan=1 << 27,
+             info=ctypes.byref(info), max_ctas=0, num_tokens=1, num_q_heads=8, num_kv_heads=2, head_dim=128, scale=0.1,
+             out=1 << 29, out_is_f32=0, lse_out=None, status=None, stream=None)
+    a.update(change)
+    assert lib.b200_paged_prefill_gqa_fp8(*a.values()) == code
+    assert b"paged_prefill_gqa_fp8" in lib.b200_last_error()

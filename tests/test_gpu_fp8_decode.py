@@ -3,13 +3,14 @@
 Tolerance.  Products of Q (exact in f16) and codes are exact and summed in fp32, the weights are
 rounded once to f16 (half a step: 2^-11 relative), the output once to bf16 (2^-8).  A weight's
 rounding moves the output by at most 2^-11 sum p |v| / l, so
-|err| <= 2^-8 |out| + 2^-11 A + fp32 noise, A = sum p |v|; the noise of sums and exp2 is taken as 2^-16 A."""
+|err| <= 2^-8 |out| + 2^-11 A + fp32 noise, A = sum p |v|; the noise of sums and exp2 is taken as 2^-16 A.
+Weights below f16's normal range add what ``smallest_weights`` derives."""
 import math
 
 import pytest
 import torch
 
-from tests.fp8_cache import as_values, attention, deal_pages, random_pool
+from tests.fp8_cache import attention, deal_pages, random_pool, smallest_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -36,6 +37,7 @@ def _check(got, lse, q, kc, vc, ks, vs, table, cu, kv, scale, base=None):
     a = _magnitude(q, kc, vc, ks, vs, table, cu, kv, scale, base)
     last = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
     tol = last * want.abs() + (2.0 ** -11 + 2.0 ** -16) * a * (1 + last)
+    tol += smallest_weights(q, kc, vc, ks, vs, table, cu, kv, scale, base) * (1 + last)
     err = (got.double() - want).abs()
     assert (err <= tol).all(), float((err / tol.clamp_min(1e-300)).max())
     empty = want_lse == -math.inf

@@ -7,38 +7,49 @@
 // token for the same arithmetic.
 //
 // The plan, the work items, the TMA ring and the merge of cut pairs are those of the 16-bit kernel
-// (one persistent CTA per SM; a producer warp; two groups of four consumer warps that take alternate
-// 64-token tiles, 16 tokens a warp).  What differs:
-//   * codes become f16 on their way from shared memory to mma.sync m16n8k16: e4m3 -> f16 is exact and
-//     one instruction per pair.  Q (bf16) is scaled per row by a power of two so that it fits f16
-//     exactly, and the weights P are f16 too, three bits more than bf16.
-//   * no element is multiplied by a scale.  K's scale is uniform over a warp's 16 tokens (pages
-//     hold 16 or more) and goes into the factor that turns a product into a log2 score.  V's scale
-//     goes into the weight, w = 2^(x + log2 s_v - M): M is the running maximum of x + log2 s_v,
-//     kept beside the running maximum m of the scores x that the row sum l refers to.  So w <= 1
-//     whatever the pages' scales are, and the largest contributions have w's 11 bits.  O is in units
-//     of 2^M and is brought to l's 2^m when the row is written.
-//   * a fragment register of four codes serves two MMA k-steps (K) or two n-tiles (V): the order of
-//     the 16 dims of a k-step and of the 16 columns of an n-tile pair is free as long as Q and the
-//     output use the same, and is taken so that ldmatrix delivers the codes in place (for V after one
-//     byte permute that pairs the tokens).  A lane ends up with four neighbouring columns of O.
-//   * the scales of a tile's pages ride with the tile: 4-byte cp.async copies that complete on the
-//     stage's barrier.
+// (one persistent CTA per SM, producer warps, eight consumer warps).  What differs:
+//   * both products are transposed, S^T = K Q^T and O^T = V^T P^T: the 16 rows of an mma.sync m16n8k16 are
+//     tokens (then columns of V), its 8 columns the query rows.  A decode step of most models has at most 8
+//     (q_len * group), and the form with the query as A would spend half of every instruction on padding;
+//     9 to 16 rows take two column tiles.
+//   * codes become f16 on their way from shared memory to the MMA: e4m3 -> f16 is exact and one instruction per
+//     pair.  Q (bf16) is scaled per row by a power of two so that it fits f16 exactly, and the weights P are f16
+//     too, three bits more than bf16.  (The e4m3 form of mma.sync converts in the same way on this part: 20 cycles a
+//     scheduler for 32 x 8 codes, two f16 MMAs take 16.)
+//   * no element is multiplied by a scale.  K's scale is uniform over 16 tokens (the least a page holds) and goes
+//     into the factor that turns a product into a log2 score.  V's scale goes into the weight,
+//     w = 2^(x + log2 s_v - M): M is the running maximum of x + log2 s_v, kept beside the running maximum m of
+//     the scores x that the row sum l refers to.  So w <= 1 whatever the pages' scales are, and the largest
+//     contributions have the most bits.  O is in units of 2^M and is brought to l's 2^m when the row is written.
+//   * M only has to be common to the eight lanes that hold a row; a vote finds the tiles that raise it, all others
+//     pass without a shuffle.  m is each lane's own until the end.
+//   * the order of the 16 dims of a k-step, and which column of V an O^T row stands for, are free as long as both
+//     operands and the output use the same, and are taken so that ldmatrix delivers K's codes in place and V's after
+//     one byte permute per register.
+//   * the scales of a tile's pages ride with the tile: 4-byte cp.async copies that complete on the stage's barrier.
+//   * a tile has half the bytes, so a producer has half the time for it: one warp took 1090 cycles a tile, where
+//     HBM delivers one in 700.  Each consumer group has a producer warp of its own.
 #include "decode_walk.cuh"
 #include "fp8.cuh"
 
+#include <type_traits>
+
 namespace b200 {
 
-constexpr int kF8Groups = 2;                 // consumer groups, alternate tiles
-constexpr int kF8Stages = 10;                // a multiple of the groups: a stage stays with one group for ever
+constexpr int kF8Groups = 4;                 // consumer groups, which take the tiles in turn
+constexpr int kF8GroupWarps = 2;             // 32 tokens of a tile each
+// A multiple of the groups: a stage stays with one group for ever.  128 KB in flight; 12 stages (192 KB) leave no L1
+// to the block table, the scales and the plan, and took 402 us instead of 366 on 8 x 131072 tokens.
+constexpr int kF8Stages = 8;
 static_assert(kF8Stages % kF8Groups == 0, "each stage must always be consumed by the same warp group");
-constexpr int kF8Warps = 4 * kF8Groups;
+constexpr int kF8Warps = kF8GroupWarps * kF8Groups;
 constexpr int kF8Consumers = kF8Warps * 32;
-constexpr int kF8Threads = kF8Consumers + 32;
+constexpr int kF8Threads = kF8Consumers + 32 * kF8Groups;        // and a producer warp per group
 constexpr int kF8TileBytes = kTileTokens * kFp8HeadDim;          // K or V tile: 64 rows of 128 bytes
 constexpr int kF8StageBytes = 2 * kF8TileBytes;
 constexpr int kF8MaxBoxes = kTileTokens / kFp8MinBlockSize;      // pages a tile can span
 constexpr int kF8SlotFloats = kMaxRows * kHeadDim;
+static_assert(kF8GroupWarps * 32 == kTileTokens && kF8Warps == 8, "the merge is written for eight warps");
 static_assert(kHeadDim == kFp8HeadDim, "one head width");
 
 struct __align__(1024) DecodeFp8Smem {
@@ -54,7 +65,7 @@ struct __align__(1024) DecodeFp8Smem {
   int merge_count;                                               // cut pairs whose last record this CTA wrote
   int merge_list[kMaxDeferred];
 };
-static_assert(sizeof(DecodeFp8Smem) + 1024 <= 227 * 1024, "shared memory budget of one CTA");
+static_assert(sizeof(DecodeFp8Smem) <= 227 * 1024, "shared memory budget of one CTA");
 
 struct DecodeFp8Params {
   const __nv_bfloat16* q;
@@ -77,23 +88,161 @@ struct DecodeFp8Params {
   float scale_log2;
 };
 
-__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// D(16x8, fp32) += A(16x16, f16, row) * B(16x8, f16, col)
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8 x 8 matrix of f16 pairs that the warp holds row by row.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t t;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  return t;
+}
+
+// What a consumer warp carries through the tiles of an item with kN column tiles of 8 query rows.  Lane
+// (quad, qlane) belongs to the rows 8 n + 2 qlane + e, e = 0, 1.
+template <int kN>
+struct RowState {
+  float o[8][kN][4];             // O^T, 16 columns of V a step: [step][n][e], columns 2 quad (+1: [2 + e])
+  float m[kN][2], l[kN][2];      // this lane's maximum of the scores, and the sum that refers to it
+  float mo[kN][2];               // the row's reference of O, the same in its eight lanes
+};
+
+// One tile's 32 tokens of this warp, as two halves of 16.
+template <int kN>
+__device__ __forceinline__ void attend_tile(RowState<kN>& st, const uint32_t (&qf)[kN][8][2], const float (&to_log2)[kN][2],
+                                            const int (&lim)[kN][2], uint32_t kbase, uint32_t vbase,
+                                            const float (&s_k)[2], const float (&s_v)[2], int tok0, int row_of,
+                                            int chunk_of) {
+  // ---- S^T = K Q^T: 16 tokens a half, eight k-steps of 16 dims
+  float s[2][kN][4];
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int n = 0; n < kN; ++n) s[half][n][0] = s[half][n][1] = s[half][n][2] = s[half][n][3] = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t kb[2][4];           // tokens 0-7 and 8-15 of the half in chunk 2j, then in chunk 2j + 1
+    ldmatrix_x4(kb[0], kbase + swz128(row_of, j * 2 + chunk_of));
+    ldmatrix_x4(kb[1], kbase + swz128(row_of + 16, j * 2 + chunk_of));
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t lo = kb[half][2 * c], hi = kb[half][2 * c + 1];
+        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)lo), a2 = e4m3x2_to_f16x2((uint16_t)(lo >> 16));
+        const uint32_t a1 = e4m3x2_to_f16x2((uint16_t)hi), a3 = e4m3x2_to_f16x2((uint16_t)(hi >> 16));
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma_f16_16816(s[half][n], a0, a1, a2, a3, qf[n][2 * j + c][0], qf[n][2 * j + c][1]);
+      }
+  }
+  // ---- scores, mask, maxima; element [half][n][2 t + e]: token quad + 8 t of the half, row e
+  const float lv[2] = {fast_log2(s_v[0]), fast_log2(s_v[1])};
+  float top_o[kN][2];
+  bool raised = false;
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float top[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float f = to_log2[n][e] * s_k[half];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float& y = s[half][n][2 * t + e];
+          y = tok0 + 16 * half + 8 * t > lim[n][e] ? -INFINITY : y * f;
+        }
+        top[half] = fmaxf(s[half][n][e], s[half][n][2 + e]);
+      }
+      top_o[n][e] = fmaxf(top[0] + lv[0], top[1] + lv[1]);
+      raised |= top_o[n][e] > st.mo[n][e];
+      const float m_new = fmaxf(st.m[n][e], fmaxf(top[0], top[1]));
+      st.l[n][e] *= fast_exp2(st.m[n][e] - (m_new == -INFINITY ? 0.f : m_new));       // m = -inf -> 0
+      st.m[n][e] = m_new;
+    }
+  if (__any_sync(0xffffffffu, raised)) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float t = top_o[n][e];
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+        const float mo_new = fmaxf(st.mo[n][e], t);
+        const float shrink = fast_exp2(st.mo[n][e] - (mo_new == -INFINITY ? 0.f : mo_new));
+        st.mo[n][e] = mo_new;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          st.o[i][n][e] *= shrink;
+          st.o[i][n][2 + e] *= shrink;
+        }
+      }
+  }
+  // ---- weights: (token, row pair) fragments to the (row, token pair) ones of the second product
+  uint32_t pf[2][kN][2];
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+    float w[2][2][2];            // [half][t][e]
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float ms = st.m[n][e] == -INFINITY ? 0.f : st.m[n][e];
+      const float os = st.mo[n][e] == -INFINITY ? 0.f : st.mo[n][e];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // w = p 2^up with p = 2^(x - m); bounded, so that a weight whose p is 0 does not become 0 * inf
+        const float up = st.m[n][e] + lv[half] - os;
+        const float c = fast_exp2(up > 126.f ? 126.f : up);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float pr = fast_exp2(s[half][n][2 * t + e] - ms);
+          st.l[n][e] += pr;
+          w[half][t][e] = pr * c;
+        }
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) pf[half][n][t] = transpose_8x8(pack_f16(w[half][t][0], w[half][t][1]));
+  }
+  // ---- O^T += V^T P^T
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {                 // two 16-byte chunks of the columns at a time
+    uint32_t vb[2][4];                          // chunk 2j: tokens 0-7, 8-15 of the half; then chunk 2j + 1
+    ldmatrix_x4_trans(vb[0], vbase + swz128(row_of, j * 2 + chunk_of));
+    ldmatrix_x4_trans(vb[1], vbase + swz128(row_of + 16, j * 2 + chunk_of));
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        // bytes (token, column) (t0,d0) (t0,d1) (t1,d0) (t1,d1) -> column d0's tokens, column d1's tokens
+        const uint32_t lo = __byte_perm(vb[half][c * 2], 0, 0x3120), hi = __byte_perm(vb[half][c * 2 + 1], 0, 0x3120);
+        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)lo), a1 = e4m3x2_to_f16x2((uint16_t)(lo >> 16));
+        const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)hi), a3 = e4m3x2_to_f16x2((uint16_t)(hi >> 16));
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma_f16_16816(st.o[2 * j + c][n], a0, a1, a2, a3, pf[half][n][0], pf[half][n][1]);
+      }
+  }
 }
 
 __global__ void __launch_bounds__(kF8Threads, 1)
 paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                             const DecodeFp8Params p) {
-  extern __shared__ uint8_t smem_raw[];
-  DecodeFp8Smem& sm = *reinterpret_cast<DecodeFp8Smem*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  DecodeFp8Smem& sm = *reinterpret_cast<DecodeFp8Smem*>(smem_raw);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  if (smem_u32(smem_raw) & 1023u) {       // the swizzled tiles need a 1024-byte aligned base
+    if (threadIdx.x == 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
+    return;
+  }
 
   // The plan is host-built and reaches the device by a copy, never by the kernel in
   // front of this one: its words may be read before the grid dependency is resolved.
@@ -111,7 +260,7 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     sm.merge_count = 0;
     for (int s = 0; s < kF8Stages; ++s) {
       mbar_init(&sm.full[s], 1 + p.boxes_per_tile);   // the TMA bytes, and each box's two scales
-      mbar_init(&sm.empty[s], 4);                     // one arrival per warp of the consuming group
+      mbar_init(&sm.empty[s], kF8GroupWarps);         // one arrival per warp of the consuming group
     }
     mbar_fence_init();
   }
@@ -145,8 +294,9 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   if (item_begin >= item_end) return;
   volatile int* abort_flag = &sm.abort_flag;
 
-  if (warp == kF8Warps) {
-    // ------------------------------ producer ------------------------------
+  if (warp >= kF8Warps) {
+    // --------------- producer of group warp - kF8Warps: its tiles, its stages ---------------
+    const int grp = warp - kF8Warps;
     if (lane == 0) {
       tma_prefetch_desc(&k_map);
       tma_prefetch_desc(&v_map);
@@ -183,6 +333,13 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         }
         continue;
       }
+      {                                              // on to this group's next tile of the item
+        const int ahead = (grp - (int)it) & (kF8Groups - 1);
+        const int step = min(ahead, w.tile_end - w.tile);
+        it += step;
+        w.tile += step;
+        if (w.tile >= w.tile_end) continue;
+      }
       const int first_lb = (w.tile * kTileTokens) >> p.block_shift;
       const int base = first_lb & ~31;
       if (w.cur.seq != win_seq || base != win_base) {
@@ -203,10 +360,8 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
 
       const int s = it % kF8Stages;
       const uint32_t ph = (it / kF8Stages) & 1u;
-      if (lane == 0) {
-        mbar_wait_bounded(&sm.empty[s], ph ^ 1u, abort_flag, p.status);
-        mbar_arrive_expect_tx(&sm.full[s], kF8StageBytes);
-      }
+      mbar_wait_bounded(&sm.empty[s], ph ^ 1u, abort_flag, p.status);
+      if (lane == 0) mbar_arrive_expect_tx(&sm.full[s], kF8StageBytes);
       __syncwarp();
       if (lane < nbox) {
         const bool have = b >= 0 && b < p.num_blocks;
@@ -230,9 +385,9 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     }
     // drain: do not leave while copies may still land in this CTA's shared memory
     if (lane == 0) {
-      const uint32_t n = it < (uint32_t)kF8Stages ? it : (uint32_t)kF8Stages;
-      for (uint32_t k = 0; k < n; ++k) {
-        const uint32_t j = it - 1 - k;
+      const uint32_t mine = (it + kF8Groups - 1 - grp) / kF8Groups;      // tiles this warp has loaded
+      for (uint32_t k = 0; k < (uint32_t)(kF8Stages / kF8Groups) && k < mine; ++k) {
+        const uint32_t j = (mine - 1 - k) * kF8Groups + grp;
         mbar_wait_bounded(&sm.full[j % kF8Stages], (j / kF8Stages) & 1u, abort_flag, p.status);
       }
     }
@@ -240,26 +395,25 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   }
 
   // -------------------------------- consumers --------------------------------
-  const int grp = warp >> 2;          // which tiles (running tile counter modulo the groups)
-  const int wslice = warp & 3;        // 16-token slice of the tile
+  const int grp = warp / kF8GroupWarps;          // which tiles (running tile counter modulo the groups)
+  const int wslice = (warp % kF8GroupWarps) * 32; // 32-token slice of the tile
   const int quad = lane >> 2;         // fragment row (and row + 8)
   const int qlane = lane & 3;
   const int G = p.group;
-  const int box = (wslice * 16) / p.box_tokens;                          // the page of this warp's tokens
+  const int box[2] = {wslice / p.box_tokens, (wslice + 16) / p.box_tokens};   // the pages of its two halves
 
   // ldmatrix lane addressing (row of the tile, which of two 16-byte chunks)
-  const int k_tok = wslice * 16 + ((lane >> 4) << 3) + (lane & 7);       // matrices 2,3 -> tokens +8
-  const int k_sel = (lane >> 3) & 1;                                     // matrices 1,3 -> next chunk
-  const int v_tok = wslice * 16 + (((lane >> 3) & 1) << 3) + (lane & 7); // matrices 1,3 -> tokens +8
-  const int v_sel = lane >> 4;                                           // matrices 2,3 -> next chunk
+  const int row_of = wslice + (((lane >> 3) & 1) << 3) + (lane & 7);     // matrices 1,3 -> tokens +8
+  const int chunk_of = lane >> 4;                                        // matrices 2,3 -> next chunk
 
   TileWalker w{items, item_begin, item_end, 0, 0, {}};
   w.set(r1, r2, r3);
   uint32_t it = 0;
 
-  // Q rows of an item as they lie in memory, 8 bytes (4 dims) per 16-dim k-step; rows beyond q_len*group
-  // are zero.  They are fetched for the NEXT item right after the tile loop, so the global loads fly
-  // while the warps merge and write the current item.
+  // Q rows of an item as they lie in memory: lane (quad, qlane) is the source of rows quad and quad + 8 in the
+  // B fragments (k = dim, n = row), 8 bytes (4 dims) per 16 dims; rows beyond q_len*group are zero.  They are fetched
+  // for the NEXT item right after the tile loop, so the global loads fly while the warps merge and write the current
+  // item.
   uint2 qraw[2][8];
   // rows of an item; none if they do not lie within q and out (a plan refilled for a larger step)
   auto rows_of = [&](const DecodeItem& qi) -> int {
@@ -312,153 +466,114 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
   while (w.item < w.item_end) {
     const DecodeItem item = w.cur;
     const int rows = rows_of(item);
-    // last visible key per fragment row (-1: row unused, everything masked)
-    const int lim[2] = {quad < rows ? min(item.causal_base + quad / G, item.kv_len - 1) : -1,
-                        quad + 8 < rows ? min(item.causal_base + (quad + 8) / G, item.kv_len - 1) : -1};
-
-    // ---- Q to f16: each row times a power of two that brings its largest magnitude to [2^14, 2^15).
-    // bf16 has 8 significant bits, f16 11 down to 2^-14: exact for all elements within 2^-28 of the
-    // row's largest, and 2^-39 of it off at most below that.
-    uint32_t qf[8][4];
-    float to_log2[2];                  // what turns a product of the row with K codes into units of log2 / s_k
+    // The item's tiles, with one column tile of query rows or two.  What they leave goes to the reduction arrays
+    // and, in `o`, to the merge below.
+    float row_m[2][2], row_l[2][2], row_o[2][2];       // of rows 8 n + 2 qlane + e
+    float o[8][2][4];
+    auto attend = [&](auto n_c) {
+      constexpr int kN = decltype(n_c)::value;
+      // Q to f16: each row times a power of two that brings its largest magnitude to [2^14, 2^15).  bf16 has 8
+      // significant bits, f16 11 down to 2^-14: exact for all elements within 2^-28 of the row's largest, and 2^-39 of it
+      // off at most below that.
+      uint32_t qf[kN][8][2];
+      float to_log2[kN][2];              // per row of this lane: a product with K codes to log2 units / s_k
+      int lim[kN][2];                    // its last visible key (-1: row unused, everything masked)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t top = 0;
+      for (int n = 0; n < kN; ++n) {
+        uint32_t top = 0;
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        top = max(top, max(qraw[h][ks].x & 0x7fffu, (qraw[h][ks].x >> 16) & 0x7fffu));
-        top = max(top, max(qraw[h][ks].y & 0x7fffu, (qraw[h][ks].y >> 16) & 0x7fffu));
-      }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = max((int)(top >> 7), 15);                      // exponent field; at least 15 keeps both factors normal
-      const float up = __uint_as_float((uint32_t)(268 - e) << 23); // 2^(14 - (e - 127))
-      to_log2[h] = __uint_as_float((uint32_t)(e - 14) << 23) * p.scale_log2;
+        for (int ks = 0; ks < 8; ++ks) {
+          top = max(top, max(qraw[n][ks].x & 0x7fffu, (qraw[n][ks].x >> 16) & 0x7fffu));
+          top = max(top, max(qraw[n][ks].y & 0x7fffu, (qraw[n][ks].y >> 16) & 0x7fffu));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int ex = max((int)(top >> 7), 15);                     // exponent field; at least 15 keeps both factors normal
+        const float up = __uint_as_float((uint32_t)(268 - ex) << 23); // 2^(14 - (ex - 127))
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        const uint2 v = qraw[h][ks];
-        qf[ks][h] = pack_f16(__uint_as_float(v.x << 16) * up, __uint_as_float(v.x & 0xffff0000u) * up);
-        qf[ks][2 + h] = pack_f16(__uint_as_float(v.y << 16) * up, __uint_as_float(v.y & 0xffff0000u) * up);
-      }
-    }
-
-    float o[16][4];                    // [16-column chunk * 2 + even / odd column][fragment]
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint2 v = qraw[n][ks];
+          qf[n][ks][0] = pack_f16(__uint_as_float(v.x << 16) * up, __uint_as_float(v.x & 0xffff0000u) * up);
+          qf[n][ks][1] = pack_f16(__uint_as_float(v.y << 16) * up, __uint_as_float(v.y & 0xffff0000u) * up);
+        }
 #pragma unroll
-    for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, mo[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-    for (int tile = item.tile_begin; tile < item.tile_end; ++tile, ++it) {
-      if ((int)(it % kF8Groups) != grp) continue;
-      const int s = it % kF8Stages;
-      mbar_wait_bounded(&sm.full[s], (it / kF8Stages) & 1u, abort_flag, p.status);
-      const uint32_t kbase = smem_u32(sm.stage[s]);
-      const uint32_t vbase = kbase + kF8TileBytes;
-      const float s_k = sm.page_scale[s][0][box], s_v = sm.page_scale[s][1][box];
-
-      // ---- S = Q K^T for this warp's 16 tokens (two n-tiles of 8); four accumulator sets shorten the
-      // chain of dependent MMAs
-      float sacc[2][2][4];
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) sacc[c][n][0] = sacc[c][n][1] = sacc[c][n][2] = sacc[c][n][3] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t kb[4];
-        ldmatrix_x4(kb, kbase + swz128(k_tok, j * 2 + k_sel));
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const uint32_t codes = kb[n * 2 + c];
-            mma_f16_16816(sacc[c][n], qf[j * 2 + c], e4m3x2_to_f16x2((uint16_t)codes),
-                          e4m3x2_to_f16x2((uint16_t)(codes >> 16)));
-          }
-      }
-      // ---- mask + online softmax (fp32, exp2 domain)
-      const int tok0 = tile * kTileTokens + wslice * 16 + qlane * 2;
-      const float lv = fast_log2(s_v);
-      float x[2][4];                   // [row][n-tile * 2 + e]
-      float w_of[2];                   // what turns p = 2^(x - m) into the weight 2^(x + lv - mo)
-      bool grown = false;
-      float shrink_o[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float f = to_log2[h] * s_k;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float y = (sacc[0][n][2 * h + e] + sacc[1][n][2 * h + e]) * f;
-            if (tok0 + n * 8 + e > lim[h]) y = -INFINITY;
-            x[h][n * 2 + e] = y;
-            mx = fmaxf(mx, y);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m[h], mx);
-        const float ms = m_new == -INFINITY ? 0.f : m_new;
-        l[h] *= fast_exp2(m[h] - ms);                              // m = -inf -> 0
-        m[h] = m_new;
-        const float mo_new = fmaxf(mo[h], mx + lv);
-        const float mos = mo_new == -INFINITY ? 0.f : mo_new;
-        shrink_o[h] = fast_exp2(mo[h] - mos);
-        grown |= mo_new != mo[h];
-        mo[h] = mo_new;
-        // bounded, so that a weight whose p is 0 does not become 0 * inf (a NaN scale stays NaN)
-        const float up = m_new + lv - mos;
-        w_of[h] = fast_exp2(up > 126.f ? 126.f : up);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[h][i] = fast_exp2(x[h][i] - ms);
-          l[h] += x[h][i];
+        for (int e = 0; e < 2; ++e) {
+          const int row = 2 * qlane + e;                             // its maximum is with the lanes of quad `row`
+          const int row_ex = __shfl_sync(0xffffffffu, ex, row * 4);
+          to_log2[n][e] = __uint_as_float((uint32_t)(row_ex - 14) << 23) * p.scale_log2;
+          lim[n][e] = 8 * n + row < rows ? min(item.causal_base + (8 * n + row) / G, item.kv_len - 1) : -1;
         }
       }
-      if (__any_sync(0xffffffffu, grown)) {
+      RowState<kN> st;
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          o[n][0] *= shrink_o[0]; o[n][1] *= shrink_o[0]; o[n][2] *= shrink_o[1]; o[n][3] *= shrink_o[1];
-        }
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) st.o[i][n][0] = st.o[i][n][1] = st.o[i][n][2] = st.o[i][n][3] = 0.f;
+        st.m[n][0] = st.m[n][1] = st.mo[n][0] = st.mo[n][1] = -INFINITY;
+        st.l[n][0] = st.l[n][1] = 0.f;
       }
-      uint32_t pf[4];
+      const uint32_t first = it + ((grp - it) & (kF8Groups - 1));    // this group's first tile of the item
+      const uint32_t last = it + (uint32_t)(item.tile_end - item.tile_begin);
+      for (uint32_t k = first; k < last; k += kF8Groups) {
+        const int tile = item.tile_begin + (int)(k - it);
+        const int s = k % kF8Stages;
+        mbar_wait_bounded(&sm.full[s], (k / kF8Stages) & 1u, abort_flag, p.status);
+        const float s_k[2] = {sm.page_scale[s][0][box[0]], sm.page_scale[s][0][box[1]]};
+        const float s_v[2] = {sm.page_scale[s][1][box[0]], sm.page_scale[s][1][box[1]]};
+        // Rows past the sequence's end carry weight 0, but 0 x NaN is NaN: whatever codes an unwritten cache slot
+        // holds must not reach the MMA.  Only a pair's last tile has such rows; the warp clears its own.
+        const bool ragged = (tile + 1) * kTileTokens > item.kv_len;
+        if (ragged) {
+          const int first_bad = item.kv_len - tile * kTileTokens;    // first row of the tile past the end
+          for (int idx = lane; idx < 32 * 8; idx += 32) {
+            const int row = wslice + (idx >> 3);
+            if (row >= first_bad)
+              *reinterpret_cast<uint4*>(sm.stage[s] + kF8TileBytes + swz128(row, idx & 7)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          __syncwarp();
+        }
+        const uint32_t kbase = smem_u32(sm.stage[s]);
+        attend_tile<kN>(st, qf, to_log2, lim, kbase, kbase + kF8TileBytes, s_k, s_v, tile * kTileTokens + wslice + quad,
+                        row_of, chunk_of);
+        // the stage goes back to TMA: order this warp's stores into it before TMA's writes
+        if (ragged) fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.empty[s]);
+      }
+      it = last;
+      // the eight lanes' own maxima and sums to the row's
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          pf[n * 2 + h] = pack_f16(x[h][n * 2] * w_of[h], x[h][n * 2 + 1] * w_of[h]);
-      // ---- rows past the sequence's end carry weight 0, but 0 x NaN is NaN: whatever codes an
-      // unwritten cache slot holds must not reach the MMA.  Only a pair's last tile has such rows;
-      // the warp clears its own 16 of them in shared memory.
-      const bool ragged = (tile + 1) * kTileTokens > item.kv_len;
-      if (ragged) {
-        const int first_bad = item.kv_len - tile * kTileTokens;          // first row of the tile past the end
-        for (int idx = lane; idx < 16 * 8; idx += 32) {
-          const int row = wslice * 16 + (idx >> 3);
-          if (row >= first_bad)
-            *reinterpret_cast<uint4*>(sm.stage[s] + kF8TileBytes + swz128(row, idx & 7)) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        __syncwarp();
-      }
-      // ---- O += P V (k = this warp's 16 tokens, n = 128 dims)
+        for (int e = 0; e < 2; ++e) {
+          float top = -INFINITY, sum = 0.f, ref = -INFINITY;
+          if (n < kN) {
+            const int nn = n < kN ? n : 0;
+            const float own = st.m[nn][e];
+            top = own;
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            sum = top == -INFINITY ? st.l[nn][e] : st.l[nn][e] * fast_exp2(own - top);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            ref = st.mo[nn][e];
+          }
+          row_m[n][e] = top;
+          row_l[n][e] = sum;
+          row_o[n][e] = ref;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t vb[4];
-        ldmatrix_x4_trans(vb, vbase + swz128(v_tok, j * 2 + v_sel));
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          // bytes (token, column): (t0,d0) (t0,d1) (t1,d0) (t1,d1) -> column d0's tokens, column d1's tokens
-          const uint32_t lo = __byte_perm(vb[c * 2], 0, 0x3120), hi = __byte_perm(vb[c * 2 + 1], 0, 0x3120);
-          const int n = (j * 2 + c) * 2;
-          mma_f16_16816(o[n], pf, e4m3x2_to_f16x2((uint16_t)lo), e4m3x2_to_f16x2((uint16_t)hi));
-          mma_f16_16816(o[n + 1], pf, e4m3x2_to_f16x2((uint16_t)(lo >> 16)), e4m3x2_to_f16x2((uint16_t)(hi >> 16)));
+          for (int i = 0; i < 8; ++i) {
+            o[i][n][e] = n < kN ? st.o[i][n < kN ? n : 0][e] : 0.f;
+            o[i][n][2 + e] = n < kN ? st.o[i][n < kN ? n : 0][2 + e] : 0.f;
+          }
         }
-      }
-      // the stage goes back to TMA: order this warp's stores into it before TMA's writes
-      if (ragged) fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.empty[s]);
-    }
+    };
+    if (rows <= 8)
+      attend(std::integral_constant<int, 1>{});
+    else
+      attend(std::integral_constant<int, 2>{});
 
     // ---- next item's Q on its way, then merge the warps (fixed order) and write the result
     ++w.item;
@@ -468,14 +583,14 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       load_q(w.cur);
     }
     if (pending_multi >= 0) __threadfence();      // stores of the PREVIOUS partial record (long done)
+    if (quad == 0) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (qlane == 0) {
-        sm.red_m[warp][quad + 8 * h] = m[h];
-        sm.red_o[warp][quad + 8 * h] = mo[h];
-      }
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          sm.red_m[warp][8 * n + 2 * qlane + e] = row_m[n][e];
+          sm.red_o[warp][8 * n + 2 * qlane + e] = row_o[n][e];
+        }
     }
     named_bar_sync(1, kF8Consumers);                           // (1) every warp's row maxima are in place
     if (pending_multi >= 0) {
@@ -484,58 +599,62 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     }
     // bring this warp's sums and accumulators to the rows' common maxima
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float g = -INFINITY, go = -INFINITY;
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int ww = 0; ww < kF8Warps; ++ww) {
-        g = fmaxf(g, sm.red_m[ww][quad + 8 * h]);
-        go = fmaxf(go, sm.red_o[ww][quad + 8 * h]);
-      }
-      const float f = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - g);
-      const float fo = mo[h] == -INFINITY ? 0.f : fast_exp2(mo[h] - go);
-      if (qlane == 0) sm.red_l[warp][quad + 8 * h] = l[h] * f;
+      for (int e = 0; e < 2; ++e) {
+        const int row = 8 * n + 2 * qlane + e;
+        float g = -INFINITY, go = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        o[n][2 * h] *= fo;
-        o[n][2 * h + 1] *= fo;
+        for (int ww = 0; ww < kF8Warps; ++ww) {
+          g = fmaxf(g, sm.red_m[ww][row]);
+          go = fmaxf(go, sm.red_o[ww][row]);
+        }
+        // a row whose scores are all NaN has no maximum but a sum that says so
+        const float f = row_m[n][e] == -INFINITY ? 1.f : fast_exp2(row_m[n][e] - g);
+        const float fo = row_o[n][e] == -INFINITY ? 1.f : fast_exp2(row_o[n][e] - go);
+        if (quad == 0) sm.red_l[warp][row] = row_l[n][e] * f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[i][n][e] *= fo;
+          o[i][n][2 + e] *= fo;
+        }
       }
-    }
-    // A lane holds four neighbouring columns of a row: 16-byte accesses, of which the eight lanes of a
-    // phase belong to two rows.  Rows are a multiple of the 32 banks apart, so odd rows have their
-    // 16-column halves swapped.
-    const int swz = (quad & 1) << 4;              // same for row quad and row quad + 8
-    if (warp >= 4 && warp < 8) {
+    // A lane holds two neighbouring columns of a row: 8-byte accesses, of which the 16 lanes of a phase belong to four
+    // rows of four quads each.  Rows are a multiple of the 32 banks apart: the column is XOR-ed with 8 times the
+    // row's lane, which spreads them over all banks.
+    const int swz = qlane << 3;
+    const int n_cols = rows > 8 ? 2 : 1;          // column tiles that hold rows
+    if (warp >= 4) {
       float* slot = sm.slots[warp - 4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int col = (c * 16 + qlane * 4) ^ swz;
-        *reinterpret_cast<float4*>(slot + quad * kHeadDim + col) =
-            make_float4(o[2 * c][0], o[2 * c + 1][0], o[2 * c][1], o[2 * c + 1][1]);
-        *reinterpret_cast<float4*>(slot + (quad + 8) * kHeadDim + col) =
-            make_float4(o[2 * c][2], o[2 * c + 1][2], o[2 * c][3], o[2 * c + 1][3]);
+      for (int n = 0; n < 2; ++n) {
+        if (n >= n_cols) break;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float2*>(slot + (8 * n + 2 * qlane + e) * kHeadDim + ((16 * i + 2 * quad) ^ swz)) =
+                make_float2(o[i][n][e], o[i][n][2 + e]);
       }
     }
     named_bar_sync(1, kF8Consumers);                           // (2) warps 4-7 have parked their sums
     if (warp < 4) {
-      // Add the partner warp's sums in place: a thread rewrites exactly the words it read.  Loads of four
-      // chunks are issued together before any of their stores (the compiler must assume they alias).
+      // Add the partner warp's sums in place: a thread rewrites exactly the words it read.  The loads of a row
+      // are issued together before any of their stores (the compiler must assume they alias).
       float* slot = sm.slots[warp];
 #pragma unroll
-      for (int c0 = 0; c0 < 8; c0 += 4) {
-        float4 a[4], b[4];
+      for (int n = 0; n < 2; ++n) {
+        if (n >= n_cols) break;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int col = ((c0 + u) * 16 + qlane * 4) ^ swz;
-          a[u] = *reinterpret_cast<const float4*>(slot + quad * kHeadDim + col);
-          b[u] = *reinterpret_cast<const float4*>(slot + (quad + 8) * kHeadDim + col);
-        }
+        for (int e = 0; e < 2; ++e) {
+          float* row_at = slot + (8 * n + 2 * qlane + e) * kHeadDim;
+          float2 a[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int c = c0 + u, col = (c * 16 + qlane * 4) ^ swz;
-          *reinterpret_cast<float4*>(slot + quad * kHeadDim + col) =
-              make_float4(a[u].x + o[2 * c][0], a[u].y + o[2 * c + 1][0], a[u].z + o[2 * c][1], a[u].w + o[2 * c + 1][1]);
-          *reinterpret_cast<float4*>(slot + (quad + 8) * kHeadDim + col) =
-              make_float4(b[u].x + o[2 * c][2], b[u].y + o[2 * c + 1][2], b[u].z + o[2 * c][3], b[u].w + o[2 * c + 1][3]);
+          for (int i = 0; i < 8; ++i) a[i] = *reinterpret_cast<const float2*>(row_at + ((16 * i + 2 * quad) ^ swz));
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float2*>(row_at + ((16 * i + 2 * quad) ^ swz)) =
+                make_float2(a[i].x + o[i][n][e], a[i].y + o[i][n][2 + e]);
         }
       }
     }
@@ -567,7 +686,7 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     for (int h = 0; h < 2; ++h) {
       const int row = (t >> 5) + h * 8;
       if (row >= rows || !record_fits) continue;
-      const int pcol = col ^ ((row & 1) << 4);
+      const int pcol = col ^ (((row >> 1) & 3) << 3);
       float4 acc = *reinterpret_cast<const float4*>(&sm.slots[0][row * kHeadDim + pcol]);
 #pragma unroll
       for (int sl = 1; sl < 4; ++sl) {
@@ -687,7 +806,7 @@ extern "C" int b200_paged_decode_gqa_fp8(const void* q, int64_t q_stride, const 
   p.out_is_f32 = out_is_f32;
   p.scale_log2 = scale * 1.4426950408889634f;
 
-  const size_t smem = sizeof(DecodeFp8Smem) + 1024;
+  const size_t smem = sizeof(DecodeFp8Smem);
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);

@@ -122,34 +122,70 @@ def reshape_and_cache(key: torch.Tensor, value: Optional[torch.Tensor],
 
 
 # --------------------------------------------------------------------------- #
+# The calls over an 8-bit cache run once per layer: their checks ask each tensor for a property once and
+# leave the error's wording to a second look.
+_E4M3, _F32, _BF16, _I32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
+_status_ptrs: dict = {}
+
+
+def _status_ptr(index: int) -> int:
+    """Address of the status word of CUDA device ``index``."""
+    if index not in _status_ptrs:
+        _status_ptrs[index] = status_word(torch.device("cuda", index)).data_ptr()
+    return _status_ptrs[index]
+
+
+def _call_on(index: int, name: str, *args) -> None:
+    """Library call ``name`` with device ``index`` current; the status word and torch's current stream of that
+    device are appended to ``args``."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _status_ptr(index), _stream_ptr(torch.device("cuda", index)) if _raw_stream is None
+                else _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _status_ptr(index), _stream_ptr(torch.device("cuda", index)))
+    if rc:
+        _lib.check(rc, name)
+
+
 def _check_fp8_cache(key_cache, value_cache, key_scale, value_scale) -> tuple:
     """(num_blocks, block_size, Hkv, D) of an 8-bit cache whose four tensors fit together."""
-    if key_cache.dtype != torch.float8_e4m3fn or value_cache.dtype != torch.float8_e4m3fn:
-        raise ValueError("8-bit KV caches hold torch.float8_e4m3fn codes")
-    if key_scale.dtype != torch.float32 or value_scale.dtype != torch.float32:
-        raise ValueError("the scales of an 8-bit KV cache are torch.float32")
     shape = key_cache.shape
+    if (key_cache.dtype is _E4M3 and value_cache.dtype is _E4M3 and key_scale.dtype is _F32
+            and value_scale.dtype is _F32 and len(shape) == 4 and value_cache.shape == shape
+            and key_scale.shape == (shape[0], shape[2]) and value_scale.shape == key_scale.shape
+            and key_cache.is_contiguous() and value_cache.is_contiguous() and key_scale.is_contiguous()
+            and value_scale.is_contiguous()):
+        return shape
+    if key_cache.dtype != _E4M3 or value_cache.dtype != _E4M3:
+        raise ValueError("8-bit KV caches hold torch.float8_e4m3fn codes")
+    if key_scale.dtype != _F32 or value_scale.dtype != _F32:
+        raise ValueError("the scales of an 8-bit KV cache are torch.float32")
     if len(shape) != 4 or value_cache.shape != shape:
         raise ValueError("8-bit KV caches must both be (num_blocks, block_size, Hkv, D)")
     if key_scale.shape != (shape[0], shape[2]) or value_scale.shape != (shape[0], shape[2]):
         raise ValueError("the scales of an 8-bit KV cache must be (num_blocks, Hkv)")
-    if not (key_cache.is_contiguous() and value_cache.is_contiguous()
-            and key_scale.is_contiguous() and value_scale.is_contiguous()):
-        raise ValueError("8-bit KV caches and their scales must be contiguous")
-    return tuple(shape)
+    raise ValueError("8-bit KV caches and their scales must be contiguous")
 
 
-def _same_device(device, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"all tensors of a call must be on one device: {device} and {t.device}")
+def _device_of(first, *others) -> int:
+    """Index of the one CUDA device all given tensors are on (None is passed over)."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _need_cuda(first, *others)
+            raise ValueError("all tensors of a call must be on one device")
+    if index < 0:
+        _need_cuda(first)
+    return index
 
 
 def _aligned_rows(x: torch.Tensor, row: int) -> torch.Tensor:
     """``x`` (T, heads, D) with its heads contiguous, tokens a multiple of 16 bytes apart and a
     16-byte aligned base: itself when it is so already, else a copy."""
-    if (x.stride(2) != 1 or x.stride(1) != x.shape[2] or x.stride(0) % 8 or x.stride(0) < row
-            or x.data_ptr() % 16):
+    token, head, dim = x.stride()
+    if dim != 1 or head != x.shape[2] or token % 8 or token < row or x.data_ptr() % 16:
         return x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -161,27 +197,24 @@ def reshape_and_cache_fp8(key: torch.Tensor, value: torch.Tensor, key_cache: tor
     codes in key_cache / value_cache (num_blocks, block_size, Hkv, 128) under the power-of-two
     scales key_scale / value_scale (num_blocks, Hkv).  A page whose first row is written starts
     anew; otherwise its scale only grows, and its other rows are then rounded to the new scale."""
-    _need_cuda(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
+    index = _device_of(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
     num_blocks, block_size, n_kv, d = _check_fp8_cache(key_cache, value_cache, key_scale, value_scale)
-    _same_device(key.device, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
-    if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
+    if key.dtype is not _BF16 or value.dtype is not _BF16:
         raise ValueError("key and value rows must be torch.bfloat16")
-    t = key.shape[0]
-    if key.shape != (t, n_kv, d) or value.shape != (t, n_kv, d):
+    shape = key.shape
+    t = shape[0]
+    if shape != (t, n_kv, d) or value.shape != shape:
         raise ValueError(f"key and value must be (T, {n_kv}, {d}) for this cache")
     if slot_mapping.shape != (t,):
         raise ValueError("slot_mapping must have one slot per token")
     if t == 0:
         return
     key, value = _aligned_rows(key, n_kv * d), _aligned_rows(value, n_kv * d)
-    if slot_mapping.dtype != torch.int32 or not slot_mapping.is_contiguous():
+    if slot_mapping.dtype is not _I32 or not slot_mapping.is_contiguous():
         slot_mapping = slot_mapping.to(torch.int32).contiguous()
-    with _on_device(key.device):
-        rc = _lib.load().b200_reshape_and_cache_fp8(
-            key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), key_cache.data_ptr(),
-            value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), slot_mapping.data_ptr(),
-            t, n_kv, d, block_size, num_blocks, status_word(key.device).data_ptr(), _stream_ptr(key.device))
-    _lib.check(rc, "b200_reshape_and_cache_fp8")
+    _call_on(index, "b200_reshape_and_cache_fp8", key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
+             key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(),
+             slot_mapping.data_ptr(), t, n_kv, d, block_size, num_blocks)
 
 
 # --------------------------------------------------------------------------- #
@@ -378,37 +411,38 @@ def paged_decode_gqa_write(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Te
 
 def _fp8_attention_args(who, q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
                         lse_out):
-    """Checks and tensors shared by the attention calls over an 8-bit cache: (q, block_table, out, cache shape)."""
-    _need_cuda(q, key_cache, value_cache, key_scale, value_scale, block_table, out, lse_out)
+    """Checks and tensors shared by the attention calls over an 8-bit cache:
+    (device index, q, block_table, out, cache shape)."""
+    index = _device_of(q, key_cache, value_cache, key_scale, value_scale, block_table, plan.dev, out, lse_out)
     shape = _check_fp8_cache(key_cache, value_cache, key_scale, value_scale)
     _, block_size, n_kv, d = shape
-    _same_device(q.device, key_cache, value_cache, key_scale, value_scale, block_table, out, lse_out, plan.dev)
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != d:
+    q_shape = q.shape
+    if q.dtype is not _BF16 or len(q_shape) != 3 or q_shape[2] != d:
         raise ValueError(f"{who}: q must be (T, Hq, {d}) torch.bfloat16")
-    t, n_q, _ = q.shape
+    t, n_q, _ = q_shape
     if n_q != plan.num_q_heads or n_kv != plan.num_kv_heads:
         raise ValueError(f"{who}: the plan was built for {plan.num_q_heads} / {plan.num_kv_heads} heads, "
                          f"the tensors have {n_q} / {n_kv}")
     if t < plan.num_tokens:
         raise ValueError(f"{who}: the plan covers {plan.num_tokens} query rows, q has {t}")
-    if block_table.dim() != 2 or block_table.shape[0] < plan.num_seqs or \
-            block_table.shape[1] * block_size < plan.max_kv:
+    table_shape = block_table.shape
+    if len(table_shape) != 2 or table_shape[0] < plan.num_seqs or table_shape[1] * block_size < plan.max_kv:
         raise ValueError(f"{who}: block_table must have {plan.num_seqs} rows of at least "
                          f"{-(-plan.max_kv // block_size)} blocks")
-    if block_table.dtype != torch.int32:
+    if block_table.dtype is not _I32:
         block_table = block_table.to(torch.int32)
-    if block_table.numel() == 0:                     # no sequence has keys: a table to point at, never read
+    if 0 in table_shape:                             # no sequence has keys: a table to point at, never read
         block_table = torch.zeros(1, 1, dtype=torch.int32, device=q.device)
     elif block_table.stride(1) != 1:
         block_table = block_table.contiguous()
     if out is None:
-        out = torch.empty(t, n_q, d, dtype=torch.float32 if out_f32 else q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype not in (torch.bfloat16, torch.float32) or not out.is_contiguous():
+        out = torch.empty_like(q, dtype=_F32 if out_f32 else _BF16, memory_format=torch.contiguous_format)
+    elif out.shape != q_shape or out.dtype not in (_BF16, _F32) or not out.is_contiguous():
         raise ValueError(f"{who}: out must be contiguous, of q's shape, torch.bfloat16 or torch.float32")
-    if lse_out is not None and (lse_out.shape != (t, n_q) or lse_out.dtype != torch.float32
+    if lse_out is not None and (lse_out.shape != (t, n_q) or lse_out.dtype is not _F32
                                 or not lse_out.is_contiguous()):
         raise ValueError(f"{who}: lse_out must be contiguous (T, Hq) torch.float32")
-    return _aligned_rows(q, n_q * d), block_table, out, shape
+    return index, _aligned_rows(q, n_q * d), block_table, out, shape
 
 
 def paged_decode_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -417,19 +451,18 @@ def paged_decode_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache: 
                          lse_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``paged_decode_gqa`` over an 8-bit cache (see ``reshape_and_cache_fp8``): the same plans, masks
     and outputs.  Rows of sequences the plan skipped are left untouched in ``out``."""
-    q, block_table, out, (num_blocks, block_size, n_kv, d) = _fp8_attention_args(
+    index, q, block_table, out, (num_blocks, block_size, n_kv, d) = _fp8_attention_args(
         "paged_decode_gqa_fp8", q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
         lse_out)
-    with _on_device(q.device):
-        rc = _lib.load().b200_paged_decode_gqa_fp8(
-            q.data_ptr(), q.stride(0), key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(),
-            value_scale.data_ptr(), num_blocks, block_size, block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[0], block_table.shape[1], plan.dev.data_ptr(),
-            None if plan.replayable else ctypes.byref(plan.info), plan.num_ctas, q.shape[0], q.shape[1], n_kv, d,
-            float(scale), plan.workspace.data_ptr(), plan.workspace.numel(), out.data_ptr(),
-            1 if out.dtype == torch.float32 else 0, lse_out.data_ptr() if lse_out is not None else None,
-            status_word(q.device).data_ptr(), _stream_ptr(q.device))
-    _lib.check(rc, "b200_paged_decode_gqa_fp8")
+    t, n_q, _ = q.shape
+    rows, cols = block_table.shape
+    workspace = plan.workspace
+    _call_on(index, "b200_paged_decode_gqa_fp8", q.data_ptr(), q.stride(0), key_cache.data_ptr(),
+             value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), num_blocks, block_size,
+             block_table.data_ptr(), block_table.stride(0), rows, cols, plan.dev.data_ptr(),
+             None if plan.replayable else ctypes.byref(plan.info), plan.num_ctas, t, n_q, n_kv, d, scale,
+             workspace.data_ptr(), workspace.numel(), out.data_ptr(), out.dtype is _F32,
+             None if lse_out is None else lse_out.data_ptr())
     return out
 
 
@@ -633,19 +666,16 @@ def paged_prefill_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache:
                           max_ctas: int = 0) -> torch.Tensor:
     """``paged_prefill_gqa`` over an 8-bit cache (see ``reshape_and_cache_fp8``): the same plans, masks
     and outputs.  Rows of sequences that are not in the plan are left untouched in ``out``."""
-    q, block_table, out, (num_blocks, block_size, n_kv, d) = _fp8_attention_args(
+    index, q, block_table, out, (num_blocks, block_size, n_kv, d) = _fp8_attention_args(
         "paged_prefill_gqa_fp8", q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
         lse_out)
-    with _on_device(q.device):
-        rc = _lib.load().b200_paged_prefill_gqa_fp8(
-            q.data_ptr(), q.stride(0), key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(),
-            value_scale.data_ptr(), num_blocks, block_size, block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[0], block_table.shape[1], plan.dev.data_ptr(),
-            None if plan.replayable else ctypes.byref(plan.info), int(max_ctas), q.shape[0], q.shape[1], n_kv, d,
-            float(scale), out.data_ptr(), 1 if out.dtype == torch.float32 else 0,
-            lse_out.data_ptr() if lse_out is not None else None,
-            status_word(q.device).data_ptr(), _stream_ptr(q.device))
-    _lib.check(rc, "b200_paged_prefill_gqa_fp8")
+    t, n_q, _ = q.shape
+    rows, cols = block_table.shape
+    _call_on(index, "b200_paged_prefill_gqa_fp8", q.data_ptr(), q.stride(0), key_cache.data_ptr(),
+             value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), num_blocks, block_size,
+             block_table.data_ptr(), block_table.stride(0), rows, cols, plan.dev.data_ptr(),
+             None if plan.replayable else ctypes.byref(plan.info), max_ctas, t, n_q, n_kv, d, scale,
+             out.data_ptr(), out.dtype is _F32, None if lse_out is None else lse_out.data_ptr())
     return out
 
 

@@ -22,8 +22,14 @@
 //   running maximum m of x.  A page is at least 16 tokens: a tile has 8 column groups of 16, each with its
 //   scales, or one pair for the whole tile when pages hold 128 tokens or more.
 //
-// Tensor-bound: flops = 4 * 128 * sum over rows of visible keys.
-#define B200_INLINE_WAITS
+// Tensor-bound: flops = 4 * 128 * sum over rows of visible keys; 1024 tensor cycles and 1024 cycles of exponentials for a
+// tile of 128 x 128, while the whole tile takes about 2100: the chain scores -> maximum -> weights -> P V of the two
+// groups over one O.  Measured (one 8-kv-head GQA layer, 32 query heads): 581 us on an 8192-token prompt (945
+// TFLOP/s), 117 us on four 512-token chunks over cached prefixes, 50 us on 5-token drafts over 2 to 8 thousand
+// tokens.  What else was tried: both groups on row tiles of their own with one K / V stream (620 us: the instruction
+// footprint of two O rescales), the groups' exponential sections kept apart by a barrier (799 us against 742 at the time).
+// All roles' loops share the SM's instruction cache, so each piece of code is instantiated once and outer loops are not
+// unrolled: from 85 KB of code to 64 KB, with the waits in line, took 742 us to 581.
 #include "fp8.cuh"
 #include "prefill_plan.cuh"
 #include "tc05.cuh"
@@ -39,9 +45,11 @@ constexpr int kP8Groups = kPfTile / kFp8MinBlockSize;           // column groups
 constexpr int kP8SoftmaxThreads = 256;
 constexpr int kP8ConvertThreads = 128;
 constexpr int kP8Threads = kP8SoftmaxThreads + 128 + kP8ConvertThreads;   // whole warpgroups: 512 = 4 x 128
-// registers per thread after the hand-over: 256 * 200 + 128 * 40 + 128 * 72 = 512 * 128
-constexpr int kP8RegsSoftmax = 200;
-constexpr int kP8RegsOther = 40;
+// Registers per thread after the hand-over: 256 * 192 + 128 * 56 + 128 * 72 = 512 * 128.  Below 56 the producer and the
+// MMA issuers spill inside their loops, which is dear where shared memory leaves no L1 (200 / 40 / 72: 123 us instead of
+// 117 on four 512-token chunks); at 192 the softmax threads do not spill.
+constexpr int kP8RegsSoftmax = 192;
+constexpr int kP8RegsOther = 56;
 constexpr int kP8RegsConvert = 72;
 constexpr int kP8TmemCols = 512;          // S0 [0,128) S1 [128,256) O [256,384) P_A [384,448) P_B [448,512)
 constexpr int kP8OCol = 256;
@@ -108,6 +116,36 @@ struct Prefill8Params {
 __host__ __device__ constexpr uint32_t umma_idesc_type0(int m, int n, bool b_mn_major) {
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// Waits for a phase of an mbarrier, at most about two seconds: the unit suspends the thread for up to a millisecond
+// at a time.  Then the CTA's abort flag goes up: every later wait returns at once, so control flow stays uniform, the
+// kernel drains to its end and reports B200_STATUS_WAIT_TIMEOUT there.  A dozen instructions: it stands at every wait
+// of loops that together have to stay in the instruction cache.
+__device__ __forceinline__ void mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t abort_at) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .u32 left, gone;\n\t"
+      "mov.u32 left, 2000;\n"
+      "again:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1, %2;\n\t"
+      "@p bra through;\n\t"
+      "ld.volatile.shared.u32 gone, [%3];\n\t"
+      "setp.ne.u32 p, gone, 0;\n\t"
+      "@p bra through;\n\t"
+      "sub.u32 left, left, 1;\n\t"
+      "setp.ne.u32 p, left, 0;\n\t"
+      "@p bra again;\n\t"
+      "st.volatile.shared.u32 [%3], 1;\n"
+      "through:\n\t}"
+      ::"r"(smem_u32(bar)), "r"(parity), "r"(1000000u), "r"(abort_at)
+      : "memory");
+}
+
+// Shared-memory matrix descriptor (128-byte swizzle) in two parts: the word with the address, and the rest.
+__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t smem_addr, uint32_t lbo_bytes) {
+  return ((smem_addr & 0x3FFFFu) >> 4) | ((lbo_bytes >> 4) & 0x3FFFu) << 16;
+}
+__host__ __device__ constexpr uint64_t umma_desc_rest(uint32_t sbo_bytes) {
+  return (uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
 // D[tmem] (+)= A[smem] * B[smem] on 8-bit codes, K = 32.
 template <bool kAccumulate>
 __device__ __forceinline__ void umma_f8_ss_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
@@ -171,10 +209,11 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
   grid_dep_wait();                // q and the step's new cache rows come from earlier kernels
   const uint32_t tmem = sm.tmem_base;
   volatile int* abort_flag = &sm.abort_flag;
+  const uint32_t abort_at = smem_u32(&sm.abort_flag);
   // Items are handed out dynamically, longest first: the producer warp draws the next index from a
   // global counter and passes it to the other roles through a two-slot mailbox.  -1 ends the CTA.
   auto take_item = [&](uint32_t k, PrefillItem& rec) -> int {
-    mbar_wait_bounded(&sm.item_full[k & 1u], (k >> 1) & 1u, abort_flag, p.status);
+    mbar_wait_limited(&sm.item_full[k & 1u], (k >> 1) & 1u, abort_at);
     const int idx = *reinterpret_cast<volatile int*>(&sm.next_item[k & 1u]);
     const int4* src = reinterpret_cast<const int4*>(&sm.next_rec[k & 1u]);
     const int4 lo = src[0], hi = src[1];
@@ -199,7 +238,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           // the first item of a CTA is its own index; the rest of the list is handed out dynamically
           idx = (k == 0) ? (int)blockIdx.x : (int)gridDim.x + atomicAdd(p.work_counter, 1);
           if (idx >= __ldg(p.work_counter - 1) || *abort_flag) idx = -1;
-          mbar_wait_bounded(&sm.item_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_flag, p.status);
+          mbar_wait_limited(&sm.item_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_at);
           if (idx >= 0) {
             const int4* src = reinterpret_cast<const int4*>(p.items + idx);
             int4* dst = reinterpret_cast<int4*>(&sm.next_rec[k & 1u]);
@@ -212,38 +251,48 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         idx = __shfl_sync(0xffffffffu, idx, 0);
         return idx;
       };
-      int idx = draw(0);
-      for (uint32_t k = 0; idx >= 0; ++k) {
-        const PrefillItem item = sm.next_rec[k & 1u];   // not overwritten before this warp draws item k + 2
+      const int groups_per_box = p.box_tokens / kFp8MinBlockSize;
+      // Each piece of code below is instantiated once: the kernel's loops share one instruction cache.  The walk
+      // starts with an item without tiles, whose only step draws item 0.
+      PrefillItem item{};
+      int idx = 0;
+#pragma unroll 1
+      for (uint32_t k = 0; idx >= 0; ++k) {          // `item` is item k - 1; item k is drawn on the way
+        const int n = item.n_tiles;
+        const int32_t* const table = p.block_table + (int64_t)item.seq * p.bt_stride;
         const int last_block = (item.kv_len - 1) >> p.block_shift;
-        const int rot = first_tile(item);
-        // Lane g < 8 looks up the page of the tile's column group g; a box is box_tokens / 16 groups.
-        // K and V travel through separate rings (a K stage is free again as soon as S = Q K^T has run), the K
-        // loads kP8KLead tiles ahead of the V loads.
-        auto issue = [&](bool is_k, int step, uint32_t itx) {
-          int tile = step + rot;
-          if (tile >= item.n_tiles) tile -= item.n_tiles;
-          int bid = -1;
-          if (lane < kP8Groups) {
-            int lb = (tile * kPfTile + lane * kFp8MinBlockSize) >> p.block_shift;
-            lb = lb > last_block ? last_block : lb;                  // the tail re-reads the last valid page
-            if (item.seq < p.table_rows && lb < p.table_cols)
-              bid = p.block_table[(int64_t)item.seq * p.bt_stride + lb];
-            if (bid >= p.num_blocks) bid = -1;
-            if (bid < 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_BLOCK);
-          }
-          const int box_bid = __shfl_sync(0xffffffffu, bid, (lane * (p.box_tokens / kFp8MinBlockSize)) & 31);
-          const int tok = (tile * kPfTile + lane * p.box_tokens) & (p.block_size - 1);
-          const int b = box_bid < 0 ? p.num_blocks : box_bid;        // outside: TMA fills zeros
-          if (is_k) {
-            const int sk = itx % kP8KStages;
-            if (lane == 0) {
-              mbar_wait_bounded(&sm.k_empty[sk], ((itx / kP8KStages) & 1u) ^ 1u, abort_flag, p.status);
-              mbar_arrive_expect_tx(&sm.k_full[sk], kP8TileBytes);
+        const int cols = item.seq < p.table_rows ? p.table_cols : 0;
+        // The next item is drawn four tiles before this one's last load: the convert warps stage its Q
+        // while this item's last tiles are worked on.
+        const int draw_at = n > 4 ? n - 4 : 0;
+        // K and V travel through separate rings (a K stage is free again as soon as S = Q K^T has run), the K loads
+        // kP8KLead tiles ahead of the V loads, which take the page ids from the K loads' look-up.
+        int ids[kP8KLead + 1];                       // of tiles step, step - 1, ..: lane g < 8 has the page of column group g
+#pragma unroll 1
+        for (int step = 0; step < n + (n > 0 ? kP8KLead : 1); ++step) {
+          if (step == draw_at) idx = draw(k);
+#pragma unroll
+          for (int i = kP8KLead; i > 0; --i) ids[i] = ids[i - 1];
+          const int box_row = lane * p.box_tokens;   // first row of this lane's box in the tile
+          if (step < n) {
+            const uint32_t itx = it + step;
+            int bid = -1;
+            if (lane < kP8Groups) {
+              int lb = (step * kPfTile + lane * kFp8MinBlockSize) >> p.block_shift;
+              lb = lb > last_block ? last_block : lb;                  // the tail re-reads the last valid page
+              if (lb < cols) bid = table[lb];
+              if (bid >= p.num_blocks) bid = -1;
+              if (bid < 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_BLOCK);
             }
+            ids[0] = bid;
+            const int b = __shfl_sync(0xffffffffu, bid, (lane * groups_per_box) & 31);
+            const int sk = itx % kP8KStages;
+            mbar_wait_limited(&sm.k_empty[sk], ((itx / kP8KStages) & 1u) ^ 1u, abort_at);
+            if (lane == 0) mbar_arrive_expect_tx(&sm.k_full[sk], kP8TileBytes);
             __syncwarp();
-            if (lane < nbox)
-              tma_load_4d(sm.k[sk] + lane * p.box_tokens * kFp8HeadDim, &k_map, &sm.k_full[sk], 0, item.kv_head, tok, b);
+            if (lane < nbox)                         // a page outside the pool: TMA fills zeros
+              tma_load_4d(sm.k[sk] + box_row * kFp8HeadDim, &k_map, &sm.k_full[sk], 0, item.kv_head,
+                          (step * kPfTile + box_row) & (p.block_size - 1), b < 0 ? p.num_blocks : b);
             // The tile's scales, through a ring of their own: the K stage is handed back before the softmax
             // threads read them.  Slot itx - 8 is free: the K stage this tile takes was freed by S of tile
             // itx - 3, whose score buffer was handed back by the readers of tile itx - 5.
@@ -254,71 +303,62 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
               cp_async_f32(&sm.tile_scale[sl][1][lane], p.scale_of[1] + at, bid >= 0);
             }
             cp_async_arrive(&sm.scale_full[sl]);
-          } else {
+          }
+          if (step >= kP8KLead && n > 0) {
+            const int tile = step - kP8KLead;
+            const uint32_t itx = it + tile;
+            const int b = __shfl_sync(0xffffffffu, ids[kP8KLead], (lane * groups_per_box) & 31);
             const int sv = itx % kP8VStages;
-            if (lane == 0) {
-              mbar_wait_bounded(&sm.v_empty[sv], ((itx / kP8VStages) & 1u) ^ 1u, abort_flag, p.status);
-              mbar_arrive_expect_tx(&sm.v_full[sv], kP8TileBytes);
-            }
+            mbar_wait_limited(&sm.v_empty[sv], ((itx / kP8VStages) & 1u) ^ 1u, abort_at);
+            if (lane == 0) mbar_arrive_expect_tx(&sm.v_full[sv], kP8TileBytes);
             __syncwarp();
             if (lane < nbox)
-              tma_load_4d(sm.v[sv] + lane * p.box_tokens * kFp8HeadDim, &v_map, &sm.v_full[sv], 0, item.kv_head, tok, b);
+              tma_load_4d(sm.v[sv] + box_row * kFp8HeadDim, &v_map, &sm.v_full[sv], 0, item.kv_head,
+                          (tile * kPfTile + box_row) & (p.block_size - 1), b < 0 ? p.num_blocks : b);
           }
           __syncwarp();
-        };
-        // The next item is drawn four tiles before this one's last load: the convert warps stage its Q
-        // while this item's last tiles are worked on.
-        int next = -1;
-        const int draw_at = item.n_tiles > 4 ? item.n_tiles - 4 : 0;
-        int kt = 0;                                  // next K tile to request
-        for (int tile = 0; tile < item.n_tiles; ++tile) {
-          if (tile == draw_at) next = draw(k + 1);
-          for (; kt < item.n_tiles && kt <= tile + kP8KLead; ++kt) issue(true, kt, it + kt);
-          issue(false, tile, it + tile);
         }
-        if (item.n_tiles == 0) next = draw(k + 1);
-        it += item.n_tiles;
-        idx = next;
+        it += n;
+        item = sm.next_rec[k & 1u];                  // not overwritten before this warp draws item k + 2
       }
       // drain: nothing may still be landing when the CTA leaves
       if (lane == 0) {
         for (uint32_t k = 0; k < (uint32_t)kP8KStages && k < it; ++k) {
           const uint32_t j = it - 1 - k;
-          mbar_wait_bounded(&sm.k_full[j % kP8KStages], (j / kP8KStages) & 1u, abort_flag, p.status);
+          mbar_wait_limited(&sm.k_full[j % kP8KStages], (j / kP8KStages) & 1u, abort_at);
         }
         for (uint32_t k = 0; k < (uint32_t)kP8VStages && k < it; ++k) {
           const uint32_t j = it - 1 - k;
-          mbar_wait_bounded(&sm.v_full[j % kP8VStages], (j / kP8VStages) & 1u, abort_flag, p.status);
+          mbar_wait_limited(&sm.v_full[j % kP8VStages], (j / kP8VStages) & 1u, abort_at);
         }
         for (uint32_t k = 0; k < (uint32_t)kP8ScaleSlots && k < it; ++k) {
           const uint32_t j = it - 1 - k;
-          mbar_wait_bounded(&sm.scale_full[j % kP8ScaleSlots], (j / kP8ScaleSlots) & 1u, abort_flag, p.status);
+          mbar_wait_limited(&sm.scale_full[j % kP8ScaleSlots], (j / kP8ScaleSlots) & 1u, abort_at);
         }
       }
     } else if (warp == 9) {
       // ------------------------- MMA issuer: S = Q K^T -------------------------
       if (lane == 0) {
         constexpr uint32_t idesc = umma_idesc_type0(kPfRows, kPfTile, false);
-        // descriptors differ only in their start-address field: build once, add offsets
-        const uint64_t dq = umma_desc_sw128(smem_u32(sm.q[0][0]), 16, 1024);
-        const uint64_t dk = umma_desc_sw128(smem_u32(sm.k[0]), 16, 1024);
-        const uint32_t dq_lo = (uint32_t)dq, dq_hi = (uint32_t)(dq >> 32);
-        const uint32_t dk_lo = (uint32_t)dk, dk_hi = (uint32_t)(dk >> 32);
+        constexpr uint32_t dq_hi = (uint32_t)(umma_desc_rest(1024) >> 32), dk_hi = dq_hi;
+        const uint32_t dq_lo = umma_desc_lo(smem_u32(sm.q[0][0]), 16), dk_lo = umma_desc_lo(smem_u32(sm.k[0]), 16);
         constexpr uint32_t kTerm = (kPfRows * kFp8HeadDim) >> 4;   // one Q term, in descriptor units
         uint32_t it = 0;
+#pragma unroll 1
         for (uint32_t item_no = 0;; ++item_no) {
           PrefillItem rec;
           if (take_item(item_no, rec) < 0) break;
           const int n_tiles = rec.n_tiles;
           const uint32_t qb = item_no & 1u;
-          mbar_wait_bounded(&sm.q_full[qb], (item_no >> 1) & 1u, abort_flag, p.status);
+          mbar_wait_limited(&sm.q_full[qb], (item_no >> 1) & 1u, abort_at);
           const uint32_t q_lo = dq_lo + qb * 2 * kTerm;
           if (n_tiles == 0) umma_commit(&sm.q_empty[qb]);
+#pragma unroll 1
           for (int tile = 0; tile < n_tiles; ++tile, ++it) {
             const int s = it % kP8KStages;
             const int b = it & 1u;
-            mbar_wait_bounded(&sm.k_full[s], (it / kP8KStages) & 1u, abort_flag, p.status);
-            mbar_wait_bounded(&sm.s_empty[b], ((it >> 1) & 1u) ^ 1u, abort_flag, p.status);
+            mbar_wait_limited(&sm.k_full[s], (it / kP8KStages) & 1u, abort_at);
+            mbar_wait_limited(&sm.s_empty[b], ((it >> 1) & 1u) ^ 1u, abort_at);
             tc_fence_after();
             const uint32_t k_lo = dk_lo + (uint32_t)((s * kP8TileBytes) >> 4);
             const uint32_t d_tmem = tmem + b * 128;
@@ -337,19 +377,21 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       // ------------------------- MMA issuer: O += P V --------------------------
       if (lane == 0) {
         constexpr uint32_t idesc = umma_idesc_type0(kPfRows, kPfHeadDim, true);
-        const uint64_t dv = umma_desc_sw128(smem_u32(sm.v16[0]), kP8TileBytes, 1024);
-        const uint32_t dv_lo = (uint32_t)dv, dv_hi = (uint32_t)(dv >> 32);
+        constexpr uint32_t dv_hi = (uint32_t)(umma_desc_rest(1024) >> 32);
+        const uint32_t dv_lo = umma_desc_lo(smem_u32(sm.v16[0]), kP8TileBytes);
         uint32_t it = 0;
+#pragma unroll 1
         for (uint32_t item_no = 0;; ++item_no) {
           PrefillItem rec;
           if (take_item(item_no, rec) < 0) break;
           const int n_tiles = rec.n_tiles;
+#pragma unroll 1
           for (int tile = 0; tile < n_tiles; ++tile, ++it) {
             const int g = it & 1u;                            // the group that owns this tile, and its V buffer
-            mbar_wait_bounded(&sm.v16_full[g], (it >> 1) & 1u, abort_flag, p.status);
-            mbar_wait_bounded(&sm.p_full[g], (it >> 1) & 1u, abort_flag, p.status);
+            mbar_wait_limited(&sm.v16_full[g], (it >> 1) & 1u, abort_at);
+            mbar_wait_limited(&sm.p_full[g], (it >> 1) & 1u, abort_at);
             if (tile == 0 && item_no > 0)                     // the previous item's O has been read
-              mbar_wait_bounded(&sm.o_free, (item_no - 1) & 1u, abort_flag, p.status);
+              mbar_wait_limited(&sm.o_free, (item_no - 1) & 1u, abort_at);
             tc_fence_after();
             const uint32_t v_lo = dv_lo + (uint32_t)((g * 2 * kP8TileBytes) >> 4);
             const uint32_t p_tmem = tmem + kP8PCol + g * 64;  // P of the tile: 128 tokens as f16 pairs
@@ -378,24 +420,25 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     const uint32_t p_col = lane_base + kP8PCol + g * 64;
     const int G = p.group;
     uint32_t it = 0;
+#pragma unroll 1
     for (uint32_t item_no = 0;; ++item_no) {
       PrefillItem item;
       if (take_item(item_no, item) < 0) break;
       const int rg = item.row0 + r;
       const bool valid = rg < item.q_len * G;
       const int lim = valid ? min(item.causal_base + rg / G, item.kv_len - 1) : -1;
-      const int rot = first_tile(item);
-      mbar_wait_bounded(&sm.q_full[item_no & 1u], (item_no >> 1) & 1u, abort_flag, p.status);
+      mbar_wait_limited(&sm.q_full[item_no & 1u], (item_no >> 1) & 1u, abort_at);
       const float row_factor = sm.row_factor[item_no & 1u][r];
       float m = -INFINITY;           // running maximum of this group's scores: what its row sum is scaled to
       float l = 0.f;
+#pragma unroll 1
       for (int tile = 0; tile < item.n_tiles; ++tile, ++it) {
         if ((int)(it & 1u) != g) continue;             // the other group's tile
         const uint32_t sb = it & 1u;
         const uint32_t s_col = lane_base + sb * 128;
         constexpr int kN = kOnePage ? 1 : kP8Groups;   // pairs of scales of a tile
         const uint32_t sl = it % kP8ScaleSlots;
-        mbar_wait_bounded(&sm.scale_full[sl], (it / kP8ScaleSlots) & 1u, abort_flag, p.status);
+        mbar_wait_limited(&sm.scale_full[sl], (it / kP8ScaleSlots) & 1u, abort_at);
         float f[kN], lv[kN];                           // product -> log2 score; log2 of V's scale
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
@@ -404,11 +447,9 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           f[i] = f[i] < 1.17549435e-38f ? 1.17549435e-38f : f[i];
           lv[i] = fast_log2(sm.tile_scale[sl][1][i]);
         }
-        mbar_wait_bounded(&sm.s_full[sb], (it >> 1) & 1u, abort_flag, p.status);
+        mbar_wait_limited(&sm.s_full[sb], (it >> 1) & 1u, abort_at);
         tc_fence_after();
-        int kv_tile = tile + rot;                      // the KV tile this step works on
-        if (kv_tile >= item.n_tiles) kv_tile -= item.n_tiles;
-        const int tbase = kv_tile * kPfTile;
+        const int tbase = tile * kPfTile;
         const bool need_mask = tbase + kPfTile - 1 > lim;
         // The whole score row goes to registers in one go and the S buffer straight back to
         // the MMA issuer.
@@ -418,7 +459,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         tmem_wait_ld();
         tc_fence_before();
         mbar_arrive(&sm.s_empty[sb]);
-        if (need_mask) {
+        if (__builtin_expect(need_mask, 0)) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4)
 #pragma unroll
@@ -453,7 +494,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         // the reference O is scaled to after the previous tile (owned by the other group)
         float m_in = -INFINITY;
         if (tile > 0) {
-          mbar_wait_bounded(&sm.m_ready[(it - 1) & 1u], ((it - 1) >> 1) & 1u, abort_flag, p.status);
+          mbar_wait_limited(&sm.m_ready[(it - 1) & 1u], ((it - 1) >> 1) & 1u, abort_at);
           m_in = sm.row_ms[(it - 1) & 1u][r];
         }
         // lazy rescale: only when some row of the warp outgrew the stale reference by 2^8
@@ -482,13 +523,13 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         // one before) has run.  The group waited for the one before that two tiles ago, so
         // the parity wait cannot be off by a phase.
         if (it >= 2) {
-          mbar_wait_bounded(&sm.pv_done[g], ((it - 2) >> 1) & 1u, abort_flag, p.status);
+          mbar_wait_limited(&sm.pv_done[g], ((it - 2) >> 1) & 1u, abort_at);
           tc_fence_after();
         }
         // O may be touched once the previous tile's P V (the other group's) has run: rare path
         if (rescale && tile > 0) {
           const float corr = (m_in == -INFINITY) ? 0.f : fast_exp2(m_in - m_used);
-          mbar_wait_bounded(&sm.pv_done[g ^ 1], ((it - 1) >> 1) & 1u, abort_flag, p.status);
+          mbar_wait_limited(&sm.pv_done[g ^ 1], ((it - 1) >> 1) & 1u, abort_at);
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
@@ -542,10 +583,10 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       // the references only grow along the tiles: the last tile's is what O is scaled to
       float mm = -INFINITY;
       if (item.n_tiles > 0) {
-        mbar_wait_bounded(&sm.m_ready[(it - 1) & 1u], ((it - 1) >> 1) & 1u, abort_flag, p.status);
+        mbar_wait_limited(&sm.m_ready[(it - 1) & 1u], ((it - 1) >> 1) & 1u, abort_at);
         mm = sm.row_ms[(it - 1) & 1u][r];
       }
-      if (item_no > 0) mbar_wait_bounded(&sm.l_empty, (item_no - 1) & 1u, abort_flag, p.status);
+      if (item_no > 0) mbar_wait_limited(&sm.l_empty, (item_no - 1) & 1u, abort_at);
       sm.row_l[g][r] = l;
       sm.row_m[g][r] = m;
       if (g == 0) sm.row_mfin[r] = mm;
@@ -586,7 +627,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       }
       const int e = max((int)(top >> 7), 8);                       // exponent field; 8 and more: both factors are normal
       const float up = __uint_as_float((uint32_t)(261 - e) << 23); // 2^(7 - (e - 127))
-      mbar_wait_bounded(&sm.q_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_flag, p.status);
+      mbar_wait_limited(&sm.q_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_at);
       uint8_t* const hi_at = sm.q[k & 1u][0];
       uint8_t* const lo_at = sm.q[k & 1u][1];
 #pragma unroll 1
@@ -617,39 +658,37 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       fence_proxy_async_smem();
       mbar_arrive(&sm.q_full[k & 1u]);
     };
-    // A thread takes the 16-byte chunk c of every 16th row: eight lanes read one row, all banks.  The 16
-    // codes become two chunks of f16, c >> 2 picks the half; lanes of the second half store their odd chunk
-    // first, so that the eight lanes of a phase again cover all banks.
-    const int c = r & 7;
+    // Bank conflicts: the eight lanes of a phase read and write 16-byte chunks of two rows, four chunks (half a row of
+    // codes) each.  Under the 128-byte swizzle a row's chunk number is XOR-ed with row & 7; rows whose numbers
+    // differ by 5 in those bits cover all banks both ways: reading, the four chunks of one row and the other four of
+    // the other (bit 2); writing 16 codes as two chunks of f16, even chunks of one row and odd ones of the other (bit 0).
+    const int pair = lane >> 3;                                    // rows {0,5}, {1,4}, {2,7}, {3,6} of each eight
+    const int row0 = (warp & 3) * 32 + (lane & 4 ? pair ^ 5 : pair);
     auto convert = [&](const PrefillItem& x, int step) {
-      int kv_tile = step + first_tile(x);
-      if (kv_tile >= x.n_tiles) kv_tile -= x.n_tiles;
-      const int have = x.kv_len - kv_tile * kPfTile;               // rows past the end are zero: 0 x NaN is NaN
+      const int have = x.kv_len - step * kPfTile;                  // rows past the end are zero: 0 x NaN is NaN
       const int sv = it % kP8VStages, b = it & 1u;
-      mbar_wait_bounded(&sm.v_full[sv], (it / kP8VStages) & 1u, abort_flag, p.status);
-      if (it >= 2) mbar_wait_bounded(&sm.pv_done[b], ((it - 2) >> 1) & 1u, abort_flag, p.status);
-      const uint8_t* src = sm.v[sv];
-      uint8_t* dst = sm.v16[b] + (c >> 2) * kP8TileBytes;
-      const int first = 2 * (c & 3) + (c >> 2), second = 2 * (c & 3) + (1 - (c >> 2));
-#pragma unroll
-      for (int i0 = 0; i0 < 8; i0 += 4) {
+      mbar_wait_limited(&sm.v_full[sv], (it / kP8VStages) & 1u, abort_at);
+      if (it >= 2) mbar_wait_limited(&sm.pv_done[b], ((it - 2) >> 1) & 1u, abort_at);
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
         uint4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = (r >> 3) + 16 * (i0 + i);
-          v[i] = *reinterpret_cast<const uint4*>(src + swz128(row, c));
-          if (row >= have) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 4; ++i)
+          v[i] = *reinterpret_cast<const uint4*>(sm.v[sv] + swz128(row0 + 8 * i, half * 4 + (lane & 3)));
+        if (have < kPfTile) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (row0 + 8 * i >= have) v[i] = make_uint4(0u, 0u, 0u, 0u);
         }
+        uint8_t* const dst = sm.v16[b] + half * kP8TileBytes;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = (r >> 3) + 16 * (i0 + i);
-          const uint4 lo = make_uint4(e4m3x2_to_f16x2((uint16_t)v[i].x), e4m3x2_to_f16x2((uint16_t)(v[i].x >> 16)),
-                                      e4m3x2_to_f16x2((uint16_t)v[i].y), e4m3x2_to_f16x2((uint16_t)(v[i].y >> 16)));
-          const uint4 hi = make_uint4(e4m3x2_to_f16x2((uint16_t)v[i].z), e4m3x2_to_f16x2((uint16_t)(v[i].z >> 16)),
-                                      e4m3x2_to_f16x2((uint16_t)v[i].w), e4m3x2_to_f16x2((uint16_t)(v[i].w >> 16)));
-          const bool odd_first = c >> 2;
-          *reinterpret_cast<uint4*>(dst + swz128(row, first)) = odd_first ? hi : lo;
-          *reinterpret_cast<uint4*>(dst + swz128(row, second)) = odd_first ? lo : hi;
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            *reinterpret_cast<uint4*>(dst + swz128(row0 + 8 * i, 2 * (lane & 3) + j)) =
+                make_uint4(e4m3x2_to_f16x2((uint16_t)w[2 * j]), e4m3x2_to_f16x2((uint16_t)(w[2 * j] >> 16)),
+                           e4m3x2_to_f16x2((uint16_t)w[2 * j + 1]), e4m3x2_to_f16x2((uint16_t)(w[2 * j + 1] >> 16)));
         }
       }
       mbar_arrive(&sm.v_empty[sv]);
@@ -657,84 +696,83 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       mbar_arrive(&sm.v16_full[b]);
       ++it;
     };
-    PrefillItem item, next;
-    int idx = take_item(0, item);
-    if (idx >= 0) {
-      stage_q(item, 0);
-      if (item.n_tiles > 0) convert(item, 0);
-    }
-    for (uint32_t item_no = 0; idx >= 0; ++item_no) {
-      // the next item's Q is staged before this item's last V tile, its first V tile right after
-      int next_idx = -1;
-      for (int tile = 1; tile < item.n_tiles; ++tile) {
-        if (tile == item.n_tiles - 1) {
-          next_idx = take_item(item_no + 1, next);
-          if (next_idx >= 0) stage_q(next, item_no + 1);
-        }
-        convert(item, tile);
-      }
-      if (item.n_tiles < 2) {
-        next_idx = take_item(item_no + 1, next);
-        if (next_idx >= 0) stage_q(next, item_no + 1);
-      }
-      if (next_idx >= 0 && next.n_tiles > 0) convert(next, 0);
-      // ---- epilogue: row e of O out of tensor memory as soon as the item's last P V has run
-      const int rg = item.row0 + r;
-      const bool valid = rg < rows_of(item);
-      const int64_t tok = item.q_start + (valid ? rg / G : 0);
-      const int head = item.kv_head * G + (valid ? rg % G : 0);
-      mbar_wait_bounded(&sm.l_full, item_no & 1u, abort_flag, p.status);
-      const float m0 = sm.row_m[0][r], m1 = sm.row_m[1][r], mo = sm.row_mfin[r];
-      const float mm = fmaxf(m0, m1);
-      // Which group had the item's even tiles depends on what the CTA worked on before: the two products
-      // are rounded alike (no fused multiply-add), so that the sum does not.
-      const float lsum = mm == -INFINITY ? sm.row_l[0][r] + sm.row_l[1][r]
-                                         : __fadd_rn(__fmul_rn(sm.row_l[0][r], fast_exp2(m0 - mm)),
-                                                     __fmul_rn(sm.row_l[1][r], fast_exp2(m1 - mm)));
-      mbar_arrive(&sm.l_empty);
-      // O is in units of 2^mo, the sum in units of 2^mm; the factor between them in two halves, each of
-      // which fp32 holds however far apart they are
-      const float half_unit = fast_exp2((mo - (mm == -INFINITY ? 0.f : mm)) * 0.5f);
-      const float inv = half_unit / lsum;
-      const bool empty = lsum == 0.f;      // no visible key: zeros, whatever the accumulator holds
-      mbar_wait_bounded(&sm.o_done, item_no & 1u, abort_flag, p.status);
-      tc_fence_after();
+    // One instance of each piece of code (see the producer): iteration k works on item k - 1, whose Q was staged in the
+    // iteration before; it stages item k before its own last V tile and writes item k - 2 behind its first.
+    PrefillItem item{}, prev{}, next{};
+    int total = -1;                                  // items of this CTA, once known
 #pragma unroll 1
-      for (int q4 = 0; q4 < 4; ++q4) {
-        uint32_t o[32];
-        tmem_ld32(o_col + q4 * 32, o);
-        tmem_wait_ld();
-        if (q4 == 3) {                       // the whole row is out of tensor memory
-          tc_fence_before();
-          mbar_arrive(&sm.o_free);
+    for (int k = 0; total < 0 || k < total + 2; ++k) {
+      const int n = item.n_tiles;
+#pragma unroll 1
+      for (int tile = 0; tile == 0 || tile < n; ++tile) {
+        if (total < 0 && tile >= n - 1) {
+          if (take_item(k, next) >= 0)
+            stage_q(next, k);
+          else
+            total = k;
         }
+        if (n > 0) convert(item, tile);
+        if (tile > 0 || k < 2) continue;
+        const uint32_t item_no = k - 2;
+        // ---- epilogue: row e of O out of tensor memory as soon as the item's last P V has run
+        const int rg = prev.row0 + r;
+        const bool valid = rg < rows_of(prev);
+        const int64_t tok = prev.q_start + (valid ? rg / G : 0);
+        const int head = prev.kv_head * G + (valid ? rg % G : 0);
+        mbar_wait_limited(&sm.l_full, item_no & 1u, abort_at);
+        const float m0 = sm.row_m[0][r], m1 = sm.row_m[1][r], mo = sm.row_mfin[r];
+        const float mm = fmaxf(m0, m1);
+        // Which group had the item's even tiles depends on what the CTA worked on before: the two products
+        // are rounded alike (no fused multiply-add), so that the sum does not.
+        const float lsum = mm == -INFINITY ? sm.row_l[0][r] + sm.row_l[1][r]
+                                           : __fadd_rn(__fmul_rn(sm.row_l[0][r], fast_exp2(m0 - mm)),
+                                                       __fmul_rn(sm.row_l[1][r], fast_exp2(m1 - mm)));
+        mbar_arrive(&sm.l_empty);
+        // O is in units of 2^mo, the sum in units of 2^mm; the factor between them in two halves, each of
+        // which fp32 holds however far apart they are
+        const float half_unit = fast_exp2((mo - (mm == -INFINITY ? 0.f : mm)) * 0.5f);
+        const float inv = half_unit / lsum;
+        const bool empty = lsum == 0.f;      // no visible key: zeros, whatever the accumulator holds
+        mbar_wait_limited(&sm.o_done, item_no & 1u, abort_at);
+        tc_fence_after();
+#pragma unroll 1
+        for (int q4 = 0; q4 < 4; ++q4) {
+          uint32_t o[32];
+          tmem_ld32(o_col + q4 * 32, o);
+          tmem_wait_ld();
+          if (q4 == 3) {                       // the whole row is out of tensor memory
+            tc_fence_before();
+            mbar_arrive(&sm.o_free);
+          }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = empty ? 0u : __float_as_uint(__uint_as_float(o[i]) * half_unit * inv);
-        if (valid) {
-          const int64_t off = (tok * p.num_q_heads + head) * kPfHeadDim + q4 * 32;
-          if (p.out_is_f32) {
-            float* dst = reinterpret_cast<float*>(p.out) + off;
+          for (int i = 0; i < 32; ++i) o[i] = empty ? 0u : __float_as_uint(__uint_as_float(o[i]) * half_unit * inv);
+          if (valid) {
+            const int64_t off = (tok * p.num_q_heads + head) * kPfHeadDim + q4 * 32;
+            if (p.out_is_f32) {
+              float* dst = reinterpret_cast<float*>(p.out) + off;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4*>(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-          } else {
-            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + off;
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4*>(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            } else {
+              __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + off;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 v;
-              v.x = pack_bf16(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
-              v.y = pack_bf16(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-              v.z = pack_bf16(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
-              v.w = pack_bf16(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
-              *reinterpret_cast<uint4*>(dst + i) = v;
+              for (int i = 0; i < 32; i += 8) {
+                uint4 v;
+                v.x = pack_bf16(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+                v.y = pack_bf16(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                v.z = pack_bf16(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
+                v.w = pack_bf16(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
+                *reinterpret_cast<uint4*>(dst + i) = v;
+              }
             }
           }
         }
+        if (valid && p.lse_out)
+          p.lse_out[tok * p.num_q_heads + head] = empty ? -INFINITY : mm * 0.6931471805599453f + __logf(lsum);
       }
-      if (valid && p.lse_out)
-        p.lse_out[tok * p.num_q_heads + head] = empty ? -INFINITY : mm * 0.6931471805599453f + __logf(lsum);
+      prev = item;
       item = next;
-      idx = next_idx;
+      if (total == k) item.n_tiles = 0;
     }
   }
   // ---- teardown: everyone is done with tensor memory before it is released
@@ -746,6 +784,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
   }
   // the last CTA to leave puts the queue back to zero for the next launch on this plan
   if (threadIdx.x == 0) {
+    if (*abort_flag && p.status) atomicOr(p.status, B200_STATUS_WAIT_TIMEOUT);
     __threadfence();
     if (atomicAdd(p.work_counter + 1, 1) == (int)gridDim.x - 1) {
       p.work_counter[0] = 0;

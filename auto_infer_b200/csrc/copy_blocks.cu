@@ -10,8 +10,10 @@ namespace b200 {
 
 constexpr int kCopyThreads = 256;
 
+// Vec: uint4, or uint32_t for pages that are no multiple of 16 bytes (the scales of an 8-bit cache).
+template <typename Vec>
 __global__ void __launch_bounds__(kCopyThreads)
-copy_blocks_kernel(const uint4* __restrict__ src, uint4* __restrict__ dst,
+copy_blocks_kernel(const Vec* __restrict__ src, Vec* __restrict__ dst,
                    const int32_t* __restrict__ src_ids, const int32_t* __restrict__ dst_ids,
                    int num_ids, int64_t page_vec, int num_src_blocks, int num_dst_blocks,
                    int chunks_per_page, int32_t* status) {
@@ -28,12 +30,12 @@ copy_blocks_kernel(const uint4* __restrict__ src, uint4* __restrict__ dst,
   const int64_t per_chunk = (page_vec + chunks_per_page - 1) / chunks_per_page;
   const int64_t lo = chunk * per_chunk;
   const int64_t hi = lo + per_chunk < page_vec ? lo + per_chunk : page_vec;
-  const uint4* sp = src + (int64_t)s * page_vec;
-  uint4* dp = dst + (int64_t)d * page_vec;
-  // four independent 16-byte loads in flight per thread
+  const Vec* sp = src + (int64_t)s * page_vec;
+  Vec* dp = dst + (int64_t)d * page_vec;
+  // four independent loads in flight per thread
   int64_t i = lo + threadIdx.x;
   for (; i + 3 * kCopyThreads < hi; i += 4 * kCopyThreads) {
-    const uint4 a = sp[i], b = sp[i + kCopyThreads], c = sp[i + 2 * kCopyThreads], e = sp[i + 3 * kCopyThreads];
+    const Vec a = sp[i], b = sp[i + kCopyThreads], c = sp[i + 2 * kCopyThreads], e = sp[i + 3 * kCopyThreads];
     dp[i] = a;
     dp[i + kCopyThreads] = b;
     dp[i + 2 * kCopyThreads] = c;
@@ -54,11 +56,12 @@ extern "C" int b200_copy_blocks(const void* src_cache, void* dst_cache, const in
     set_last_error("copy_blocks: null pointer or non-positive size");
     return B200_EINVAL;
   }
-  if (page_bytes % 16 || reinterpret_cast<uintptr_t>(src_cache) % 16 || reinterpret_cast<uintptr_t>(dst_cache) % 16) {
-    set_last_error("copy_blocks: page size and cache bases must be multiples of 16 bytes");
+  const uint64_t low = (uint64_t)page_bytes | reinterpret_cast<uintptr_t>(src_cache) | reinterpret_cast<uintptr_t>(dst_cache);
+  if (low % 4) {
+    set_last_error("copy_blocks: page size and cache bases must be multiples of 4 bytes");
     return B200_EALIGN;
   }
-  const int64_t page_vec = page_bytes / 16;
+  const bool wide = low % 16 == 0;
   // enough CTAs to fill the machine also when few pages move: a page is cut into chunks of
   // at least 16 KiB
   int chunks = 1;
@@ -70,9 +73,12 @@ extern "C" int b200_copy_blocks(const void* src_cache, void* dst_cache, const in
     set_last_error("copy_blocks: %d pages exceed one launch", num_ids);
     return B200_ETOOLARGE;
   }
-  return check_cuda(launch_pdl(copy_blocks_kernel, dim3((unsigned)grid), dim3(kCopyThreads), 0,
-                               static_cast<cudaStream_t>(stream), (const uint4*)src_cache, (uint4*)dst_cache,
-                               src_block_ids, dst_block_ids, num_ids, page_vec, num_src_blocks, num_dst_blocks,
-                               chunks, status),
-                    "copy_blocks launch");
+  auto launch = [&](auto vec) {
+    using Vec = decltype(vec);
+    return launch_pdl(copy_blocks_kernel<Vec>, dim3((unsigned)grid), dim3(kCopyThreads), 0,
+                      static_cast<cudaStream_t>(stream), (const Vec*)src_cache, (Vec*)dst_cache, src_block_ids,
+                      dst_block_ids, num_ids, page_bytes / (int64_t)sizeof(Vec), num_src_blocks, num_dst_blocks, chunks,
+                      status);
+  };
+  return check_cuda(wide ? launch(uint4{}) : launch(uint32_t{}), "copy_blocks launch");
 }

@@ -38,7 +38,7 @@ struct GqaRopeParams {
   __nv_bfloat16* q_out;
   int64_t q_out_stride;
   __nv_bfloat16* k_out;                        // (T, Hkv, 128) or null
-  __nv_bfloat16* key_cache;
+  __nv_bfloat16* key_cache;                    // null: no slot write (k_out is set)
   __nv_bfloat16* value_cache;
   const int32_t* slot_mapping;
   int num_tokens, num_q_heads, num_kv_heads;
@@ -96,6 +96,7 @@ gqa_rope_cache_kernel(const GqaRopeParams p) {
     return;
   }
   if (p.k_out) *reinterpret_cast<uint2*>(p.k_out + ((int64_t)t * p.num_kv_heads + hk) * 128 + lane * 4) = packed;
+  if (!p.key_cache) return;
   const int64_t slot = p.slot_mapping[t];
   if (slot < 0) return;                                        // padding row
   if (slot >= p.total_slots) {
@@ -228,8 +229,9 @@ extern "C" int b200_gqa_rope_cache(const void* q, int64_t q_stride, const void* 
                                    int num_blocks, int32_t* status, void* stream) {
   using namespace b200;
   if (num_tokens == 0) return B200_OK;
-  if (!q || !k || !v || !cos || !sin || !q_out || !key_cache || !value_cache || !slot_mapping ||
-      num_tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || block_size <= 0 || num_blocks <= 0 ||
+  const bool no_write = !key_cache && !value_cache && !slot_mapping && k_out;   // the caller writes the rotated keys
+  if (!q || !k || !cos || !sin || !q_out || num_tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      (!no_write && (!v || !key_cache || !value_cache || !slot_mapping || block_size <= 0 || num_blocks <= 0)) ||
       (q_norm_weight == nullptr) != (k_norm_weight == nullptr)) {
     set_last_error("gqa_rope_cache: null pointer, non-positive size, or only one of the two norm weights");
     return B200_EINVAL;

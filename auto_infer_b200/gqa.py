@@ -28,6 +28,7 @@ class B200GqaBackend(AttentionBackend):
 
     _one_launch_step = True           # paged_attention may fold the slot write into the attention launch
     _overlap_mixed = True             # a mixed step may run its two kernels side by side on disjoint SMs
+    _kv_elem_bytes = 2
 
     def __init__(self, n_q_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                  num_layers: int, device, dtype, w: dict = None, layer_prefix=None, rms_eps=None,
@@ -59,6 +60,18 @@ class B200GqaBackend(AttentionBackend):
         return [torch.zeros(shape, device=self.device, dtype=self.dtype)
                 for _ in range(self.num_layers)]
 
+    # -- the launches that depend on the cache's layout ----------------------
+    def _prologue(self, layer_idx: int, q, k, v, ctx, q_norm_weight, k_norm_weight, eps) -> torch.Tensor:
+        cache = ctx.kv_caches[layer_idx]
+        return ops.gqa_rope_cache(q, k, v, ctx.cos, ctx.sin, cache[0], cache[1], ctx.slot_mapping,
+                                  q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, eps=eps)
+
+    def _launch_decode(self, q, cache, ctx, plan, out) -> None:
+        ops.paged_decode_gqa(q, cache[0], cache[1], ctx.block_table, plan, self.scale, out=out)
+
+    def _launch_prefill(self, q, cache, ctx, plan, out, max_ctas: int = 0) -> None:
+        ops.paged_prefill_gqa(q, cache[0], cache[1], ctx.block_table, plan, self.scale, out=out, max_ctas=max_ctas)
+
     # -- whole sub-block ----------------------------------------------------
     def attention(self, layer_idx: int, x: torch.Tensor, ctx) -> torch.Tensor:
         """The sub-block of auto_infer/layers/attention/gqa.py:27-49 (its wiring is the plug-in
@@ -72,12 +85,10 @@ class B200GqaBackend(AttentionBackend):
         p = self.layer_prefix(layer_idx) + "self_attn."
         qkv = _lin(x, w[p + "qkv_proj.weight"], w.get(p + "qkv_proj.bias"))
         q, k, v = qkv.split((n_q * hd, n_kv * hd, n_kv * hd), dim=-1)
-        cache = ctx.kv_caches[layer_idx]
         qn = w.get(p + "q_norm.weight")
-        q = ops.gqa_rope_cache(q.view(t, n_q, hd), k.view(t, n_kv, hd), v.view(t, n_kv, hd), ctx.cos, ctx.sin,
-                               cache[0], cache[1], ctx.slot_mapping, q_norm_weight=qn,
-                               k_norm_weight=w[p + "k_norm.weight"] if qn is not None else None,
-                               eps=self.rms_eps if self.rms_eps is not None else 1e-6)
+        q = self._prologue(layer_idx, q.view(t, n_q, hd), k.view(t, n_kv, hd), v.view(t, n_kv, hd), ctx, qn,
+                           w[p + "k_norm.weight"] if qn is not None else None,
+                           self.rms_eps if self.rms_eps is not None else 1e-6)
         o = self._attn(layer_idx, q, None, None, ctx).reshape(t, n_q * hd)
         out = _lin(o, w[p + "o_proj.weight"])
         if self.tp_group is not None and torch.distributed.get_world_size(self.tp_group) > 1:
@@ -93,7 +104,8 @@ class B200GqaBackend(AttentionBackend):
               ctx) -> torch.Tensor:
         cache = ctx.kv_caches[layer_idx]
         meta = step_metadata(ctx, self.n_q_heads, self.n_kv_heads, self.head_dim, q.device,
-                             pool=self._meta_pool, split_mixed=self._overlap_mixed)
+                             pool=self._meta_pool, split_mixed=self._overlap_mixed,
+                             kv_elem_bytes=self._kv_elem_bytes)
         out = torch.empty(q.shape[0], self.n_q_heads, self.head_dim, dtype=q.dtype, device=q.device)
         if meta.prefill is not None and meta.prefill_ctas and meta.decode.info.num_items:
             # A mixed step, side by side: the wide-query kernel (tensor pipe, shared memory) on
@@ -106,18 +118,15 @@ class B200GqaBackend(AttentionBackend):
             fork.record(cur)
             self._side_stream.wait_event(fork)
             with torch.cuda.stream(self._side_stream):
-                ops.paged_prefill_gqa(q, cache[0], cache[1], ctx.block_table, meta.prefill, self.scale,
-                                      out=out, max_ctas=meta.prefill_ctas)
+                self._launch_prefill(q, cache, ctx, meta.prefill, out, max_ctas=meta.prefill_ctas)
                 join.record(self._side_stream)
-            ops.paged_decode_gqa(q, cache[0], cache[1], ctx.block_table, meta.decode, self.scale, out=out)
+            self._launch_decode(q, cache, ctx, meta.decode, out)
             cur.wait_event(join)
             return out
         if meta.decode.info.num_items:
-            ops.paged_decode_gqa(q, cache[0], cache[1], ctx.block_table, meta.decode, self.scale,
-                                 out=out)
+            self._launch_decode(q, cache, ctx, meta.decode, out)
         if meta.prefill is not None:
-            ops.paged_prefill_gqa(q, cache[0], cache[1], ctx.block_table, meta.prefill, self.scale,
-                                  out=out)
+            self._launch_prefill(q, cache, ctx, meta.prefill, out)
         return out
 
     def paged_attention(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -128,7 +137,8 @@ class B200GqaBackend(AttentionBackend):
         stores the new rows itself."""
         cache = ctx.kv_caches[layer_idx]
         meta = step_metadata(ctx, self.n_q_heads, self.n_kv_heads, self.head_dim, q.device,
-                             pool=self._meta_pool, split_mixed=self._overlap_mixed)
+                             pool=self._meta_pool, split_mixed=self._overlap_mixed,
+                             kv_elem_bytes=self._kv_elem_bytes)
         if meta.prefill is None and meta.decode.info.num_items and self._one_launch_step:
             return ops.paged_decode_gqa_write(q, k, v, ctx.slot_mapping, cache[0], cache[1], ctx.block_table,
                                               meta.decode, self.scale)
@@ -211,9 +221,9 @@ class B200GraphGqaBackend(B200GqaBackend):
                 del self._meta_pool[key]
         cache = ctx.kv_caches[layer_idx]
         out = torch.empty(q.shape[0], self.n_q_heads, self.head_dim, dtype=q.dtype, device=q.device)
-        ops.paged_decode_gqa(q, cache[0], cache[1], ctx.block_table, meta.decode, self.scale, out=out)
+        self._launch_decode(q, cache, ctx, meta.decode, out)
         if meta.prefill is not None:                # a prefill gear: both launches are recorded
-            ops.paged_prefill_gqa(q, cache[0], cache[1], ctx.block_table, meta.prefill, self.scale, out=out)
+            self._launch_prefill(q, cache, ctx, meta.prefill, out)
         self.reg.append(_GraphRegistration(meta, layer_idx, q, out, cache[0].shape[1]))
         return out
 
@@ -247,3 +257,50 @@ class B200GraphGqaBackend(B200GqaBackend):
             if id(registration.meta) not in seen:
                 seen.add(id(registration.meta))
                 self._refill(registration.meta, ctx, stream)
+
+
+class _Fp8Cache:
+    """What a GQA backend does differently over an 8-bit cache (``ops.reshape_and_cache_fp8``): the
+    layers' caches, the slot write (a launch of its own: a page's scale depends on all rows the
+    step brings to it), and the attention launches.  Cache memory and its traffic are half of the
+    16-bit backend's; plans, contexts and the capture protocol are the same."""
+
+    _one_launch_step = False
+    _kv_elem_bytes = 1
+
+    def alloc_kv_caches(self, num_blocks: int, block_size: int) -> list:
+        """Per layer (key codes, value codes, key scales, value scales): e4m3
+        (num_blocks, block_size, n_kv, 128) and fp32 (num_blocks, n_kv), all zeros (a scale of 0: a
+        page that was never written)."""
+        if self.dtype != torch.bfloat16 or self.head_dim != 128:
+            raise NotImplementedError("the B200 kernels over an 8-bit cache are built for bf16 models with heads of 128")
+        if num_blocks and (block_size < 16 or block_size > 1024 or block_size & (block_size - 1)):
+            raise ValueError("an 8-bit cache has pages of a power of two of 16 to 1024 tokens")
+        codes, scales = (num_blocks, block_size, self.n_kv_heads, self.head_dim), (num_blocks, self.n_kv_heads)
+        return [(torch.zeros(codes, device=self.device, dtype=torch.float8_e4m3fn),
+                 torch.zeros(codes, device=self.device, dtype=torch.float8_e4m3fn),
+                 torch.zeros(scales, device=self.device), torch.zeros(scales, device=self.device))
+                for _ in range(self.num_layers)]
+
+    def _prologue(self, layer_idx: int, q, k, v, ctx, q_norm_weight, k_norm_weight, eps) -> torch.Tensor:
+        q, k = ops.gqa_rope_cache(q, k, v, ctx.cos, ctx.sin, None, None, None, q_norm_weight=q_norm_weight,
+                                  k_norm_weight=k_norm_weight, eps=eps, want_k=True)
+        self._write_kv(layer_idx, k, v, ctx)
+        return q
+
+    def _write_kv(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, ctx) -> None:
+        ops.reshape_and_cache_fp8(k, v, *ctx.kv_caches[layer_idx], ctx.slot_mapping)
+
+    def _launch_decode(self, q, cache, ctx, plan, out) -> None:
+        ops.paged_decode_gqa_fp8(q, *cache, ctx.block_table, plan, self.scale, out=out)
+
+    def _launch_prefill(self, q, cache, ctx, plan, out, max_ctas: int = 0) -> None:
+        ops.paged_prefill_gqa_fp8(q, *cache, ctx.block_table, plan, self.scale, out=out, max_ctas=max_ctas)
+
+
+class B200Fp8GqaBackend(_Fp8Cache, B200GqaBackend):
+    """``B200GqaBackend`` over an 8-bit cache."""
+
+
+class B200GraphFp8GqaBackend(_Fp8Cache, B200GraphGqaBackend):
+    """``B200GraphGqaBackend`` over an 8-bit cache."""

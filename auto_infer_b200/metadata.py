@@ -16,26 +16,27 @@ _ATTR = "_b200_step_meta"
 
 # A mixed step (decode rows + prefill chunks) may run its two kernels side by side on disjoint
 # SMs: the decode kernel is bound by memory bandwidth, the wide-query kernel by the tensor pipe
-# and shared memory.  Cost model, measured on the part: a decode CTA streaming beside the
-# wide-query kernel moves about 53 GB/s (all of them together at most the copy bandwidth); one
-# 128 x 128 tile of the wide-query kernel takes about 1.26 us on one SM.
-_HBM_GBS = 6450.0
-_DECODE_GBS_PER_SM = 53.0
-_PREFILL_US_PER_TILE = 1.26
+# and shared memory.  Cost model, measured on the part, per size of a cache element: what all decode
+# CTAs together move (GB/s), what one moves beside the wide-query kernel (GB/s), and how long one SM
+# works on a 128 x 128 tile of the wide-query kernel (us).  The 8-bit kernels' figures are
+# fits to 24 to 120 SMs each on five mixes of 16 to 128 decode rows with 256 to 8192 new prompt tokens; of those,
+# side by side wins most on 60 decode rows beside one 256-token chunk (130 us, 160 one after the other).
+_RATES = {2: (6450.0, 53.0, 1.26), 1: (5500.0, 48.0, 1.30)}
 _DECODE_FIXED_US, _PREFILL_FIXED_US = 6.0, 4.0
 
 
 def mixed_split(decode_bytes: int, prefill_tiles: int, sms: int, prefill_items: int = 0,
-                longest_item_tiles: int = 0) -> int:
+                longest_item_tiles: int = 0, kv_elem_bytes: int = 2) -> int:
     """SMs to give the wide-query kernel in a mixed step (a multiple of 8), or 0 when running the
     two kernels one after the other on all SMs is expected to be as fast (within 7 %).  The
     wide-query kernel's work comes in items of 128 query rows (``prefill_items`` of them, the
     longest ``longest_item_tiles`` tiles): with few items per SM the longest ones set its time."""
     if decode_bytes <= 0 or prefill_tiles <= 0 or sms < 32:
         return 0
+    all_gbs, sm_gbs, us_per_tile = _RATES[kv_elem_bytes]
 
     def t_dec(n):
-        return decode_bytes / (min(_HBM_GBS, n * _DECODE_GBS_PER_SM) * 1e3) + _DECODE_FIXED_US
+        return decode_bytes / (min(all_gbs, n * sm_gbs) * 1e3) + _DECODE_FIXED_US
 
     def t_pre(n):
         tiles = prefill_tiles / n
@@ -45,7 +46,7 @@ def mixed_split(decode_bytes: int, prefill_tiles: int, sms: int, prefill_items: 
                 tiles = max(tiles, longest_item_tiles * rounds)
             else:
                 tiles += longest_item_tiles / 2
-        return tiles * _PREFILL_US_PER_TILE + _PREFILL_FIXED_US
+        return tiles * us_per_tile + _PREFILL_FIXED_US
 
     one_after_the_other = t_dec(sms) + t_pre(sms)
     best_n, best_t = 0, one_after_the_other
@@ -165,7 +166,7 @@ def cached_step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int
 
 def step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int, device,
                   causal_base: Optional[Sequence[int]] = None, pool: Optional[dict] = None,
-                  split_mixed: bool = False) -> StepMetadata:
+                  split_mixed: bool = False, kv_elem_bytes: int = 2) -> StepMetadata:
     """Fetch (or build and attach) the metadata of ``ctx`` for this head
     geometry.  The context is a plain mutable dataclass in the reference
     (auto_infer/forward_context.py:9), which already carries per-step extras
@@ -177,7 +178,8 @@ def step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int, devic
     that overlap on the GPU must run on one stream.
 
     ``split_mixed``: a step with both decode rows and prefill chunks is planned for running its
-    two kernels side by side when ``mixed_split`` expects a gain (``meta.prefill_ctas`` > 0)."""
+    two kernels side by side when ``mixed_split`` expects a gain (``meta.prefill_ctas`` > 0);
+    ``kv_elem_bytes`` is the size of a cache element."""
     cache = getattr(ctx, _ATTR, None)
     if cache is None:
         cache = {}
@@ -189,8 +191,8 @@ def step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int, devic
         if split_mixed and torch.device(device).type == "cuda":
             _, decode_bytes, prefill_tiles, items, longest = scan_step(
                 ctx.cu_seqlens_q, ctx.seqlens_kv, num_q_heads, num_kv_heads, head_dim, causal_base)
-            prefill_ctas = mixed_split(decode_bytes, prefill_tiles, ops.sm_count(torch.device(device)),
-                                       items, longest)
+            prefill_ctas = mixed_split(decode_bytes * kv_elem_bytes // 2, prefill_tiles, ops.sm_count(torch.device(device)),
+                                       items, longest, kv_elem_bytes)
         pool_key = key + (prefill_ctas,)           # a plan is built for one share of the SMs
         pooled = pool.get(pool_key) if pool is not None else None
         if pooled is not None and pooled.capacity_seqs >= len(ctx.cu_seqlens_q):

@@ -803,8 +803,8 @@ def _cache_tensors(layer):
 def copy_blocks(source_caches, target_caches, block_ids, target_block_ids=None) -> None:
     """Copy selected physical blocks between caches with identical layouts; same contract as
     ``copy_blocks`` of auto_infer/pd/connector.py:30-51 (a tensor cache is the dense
-    ``(2, blocks, ...)`` layout, a tuple holds separate key / value tensors whose leading
-    axis is the block axis), one kernel launch per cache tensor instead of one copy per
+    ``(2, blocks, ...)`` layout, a tuple holds separate tensors - key, value, the scales of an
+    8-bit cache - whose leading axis is the block axis), one kernel launch per cache tensor instead of one copy per
     block.  ``target_block_ids`` (optional, beyond the reference) lands the pages on other
     block ids of the target pool."""
     if len(source_caches) != len(target_caches):
@@ -832,6 +832,8 @@ def copy_blocks(source_caches, target_caches, block_ids, target_block_ids=None) 
                 target.shape[:block_axis] + target.shape[block_axis + 1:])
             if not same:
                 raise ValueError("source and target cache shapes must match")
+            if source.dtype != target.dtype:
+                raise ValueError("source and target cache types must match")
             _need_cuda(source, target)
             if not (source.is_contiguous() and target.is_contiguous()):
                 raise ValueError("caches must be contiguous")
@@ -852,14 +854,19 @@ def copy_blocks(source_caches, target_caches, block_ids, target_block_ids=None) 
 
 
 def gqa_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
-                   key_cache: torch.Tensor, value_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                   key_cache: Optional[torch.Tensor], value_cache: Optional[torch.Tensor],
+                   slot_mapping: Optional[torch.Tensor],
                    q_norm_weight: Optional[torch.Tensor] = None, k_norm_weight: Optional[torch.Tensor] = None,
                    eps: float = 1e-6, want_k: bool = False):
     """Fused prologue of the GQA sub-block (auto_infer/layers/attention/gqa.py:40-47): optional
     per-head RMSNorm of q / k, NeoX rotary embedding of q / k, slot write of k and v.
     q / k / v are (T, H*, 128) views (of the packed projection, typically); returns the rotated
-    q (T, Hq, 128) and, with ``want_k``, the rotated k."""
-    _need_cuda(q, k, v, cos, sin, key_cache, value_cache, slot_mapping)
+    q (T, Hq, 128) and, with ``want_k``, the rotated k.  Without caches and slots (all three None,
+    ``want_k``) nothing is written: an 8-bit cache takes the rotated k in a call of its own."""
+    write = key_cache is not None
+    if write != (value_cache is not None) or write != (slot_mapping is not None) or not (write or want_k):
+        raise ValueError("caches and slot_mapping go together, and without them want_k must be set")
+    _need_cuda(q, k, v, cos, sin, *((key_cache, value_cache, slot_mapping) if write else ()))
     lib = _lib.load()
     t, n_q, d = q.shape
     n_kv = k.shape[1]
@@ -868,13 +875,14 @@ def gqa_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch
             raise ValueError(f"{name}: each token's heads must be contiguous")
     if cos.stride(-1) != 1 or sin.stride(-1) != 1 or cos.stride(0) != sin.stride(0):
         raise ValueError("cos / sin must be (T, 1, D) with contiguous rows and equal token strides")
-    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
-        raise ValueError("KV caches must be contiguous (num_blocks, block_size, Hkv, D)")
-    if slot_mapping.dtype != torch.int32:
-        slot_mapping = slot_mapping.to(torch.int32)
+    num_blocks = block_size = 0
+    if write:
+        if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise ValueError("KV caches must be contiguous (num_blocks, block_size, Hkv, D)")
+        slot_mapping = slot_mapping.to(torch.int32).contiguous()
+        num_blocks, block_size = key_cache.shape[0], key_cache.shape[1]
     q_out = torch.empty(t, n_q, d, dtype=q.dtype, device=q.device)
     k_out = torch.empty(t, n_kv, d, dtype=k.dtype, device=k.device) if want_k else None
-    num_blocks, block_size = key_cache.shape[0], key_cache.shape[1]
     with _on_device(q.device):
         rc = lib.b200_gqa_rope_cache(
             q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
@@ -882,7 +890,7 @@ def gqa_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch
             q_norm_weight.data_ptr() if q_norm_weight is not None else None,
             k_norm_weight.data_ptr() if k_norm_weight is not None else None, float(eps),
             q_out.data_ptr(), q_out.stride(0), k_out.data_ptr() if k_out is not None else None,
-            key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.contiguous().data_ptr(),
+            *((x.data_ptr() if write else None) for x in (key_cache, value_cache, slot_mapping)),
             t, n_q, n_kv, d, block_size, num_blocks, status_word(q.device).data_ptr(), _stream_ptr(q.device))
     _lib.check(rc, "b200_gqa_rope_cache")
     return (q_out, k_out) if want_k else q_out

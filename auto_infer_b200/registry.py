@@ -37,26 +37,36 @@ def _dense_unavailable(family: str):
         "DenseBackend / MlaDenseBackend for it (install_into_auto_infer() routes it there)")
 
 
-def _gqa(model, mode: str):
-    from .gqa import B200GqaBackend, B200GraphGqaBackend
-    if mode == "dense":
-        _dense_unavailable("gqa")
-    cfg = model.cfg
+def _gqa_class(model, mode: str):
+    """The GQA backend for a model and mode.  A model that sets ``_gqa_b200_kv_dtype`` to
+    ``torch.float8_e4m3fn`` gets 8-bit caches (half the memory and traffic per token)."""
+    import torch
+    from . import gqa
+    dtype = getattr(model, "_gqa_b200_kv_dtype", torch.bfloat16)
     # "graph": the same kernels behind the lifecycle surface the graph runners drive
     # (auto_infer/layers/attention/gqa.py:134-226); lengths are read from a refillable plan
     # in device memory, so a replay needs one plan refill instead of a per-layer re-issue.
-    cls = B200GraphGqaBackend if mode == "graph" else B200GqaBackend
-    return cls(
+    graph = mode == "graph"
+    if dtype is torch.bfloat16:
+        return gqa.B200GraphGqaBackend if graph else gqa.B200GqaBackend
+    if dtype is torch.float8_e4m3fn:
+        return gqa.B200GraphFp8GqaBackend if graph else gqa.B200Fp8GqaBackend
+    raise ValueError(f"gqa: unsupported _gqa_b200_kv_dtype {dtype}; torch.bfloat16 or torch.float8_e4m3fn")
+
+
+def _gqa(model, mode: str):
+    if mode == "dense":
+        _dense_unavailable("gqa")
+    cfg = model.cfg
+    return _gqa_class(model, mode)(
         n_q_heads=model.n_q_local, n_kv_heads=model.n_kv_local, head_dim=cfg.head_dim,
         scale=cfg.head_dim ** -0.5, num_layers=cfg.num_layers, device=model.device,
         dtype=model.dtype, w=model.w, layer_prefix=model.layer_prefix, rms_eps=cfg.rms_eps)
 
 
 def _gqa_mtp(model, mode: str, prefix: str):
-    from .gqa import B200GqaBackend, B200GraphGqaBackend
     cfg = model.cfg
-    cls = B200GraphGqaBackend if mode == "graph" else B200GqaBackend
-    return cls(
+    return _gqa_class(model, mode)(
         n_q_heads=model.n_q_local, n_kv_heads=model.n_kv_local, head_dim=cfg.head_dim,
         scale=cfg.head_dim ** -0.5, num_layers=1, device=model.device, dtype=model.dtype,
         w=model.w, layer_prefix=lambda _: prefix, rms_eps=cfg.rms_eps)

@@ -551,7 +551,8 @@ int b200_cp_exchange_combine(const float* local_record, const uint64_t* recv_ptr
  *   q_norm_weight / k_norm_weight: (128) bf16, both or neither
  *   q_out (T, Hq, 128) bf16 (token stride q_out_stride): the rotated queries
  *   k_out (T, Hkv, 128) bf16 or NULL: the rotated keys, for callers that want them
- *   caches / slot_mapping: as b200_reshape_and_cache
+ *   caches / slot_mapping: as b200_reshape_and_cache; all three NULL with a k_out: no slot
+ *     write, the caller puts k_out and v elsewhere (b200_reshape_and_cache_fp8); v may be NULL then
  * Rounds to bf16 where the eager chain of bf16 tensors does, so q_out and the
  * cache rows equal that chain's. */
 int b200_gqa_rope_cache(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
@@ -589,8 +590,9 @@ int b200_mla_rope_norm_cache(const void* ckv_full, int64_t ckv_stride,
  * src_block_ids[i] of src_cache to block dst_block_ids[i] of dst_cache
  * (dst_block_ids NULL = the same ids, the reference's form).  The two caches
  * may sit on different GPUs of a node if one of them is peer-mapped into the
- * current device.  page_bytes = block_size * Hkv * dim * 2 must be a multiple of
- * 16.  Ids outside a pool are skipped and set B200_STATUS_BAD_BLOCK.  Bit-exact. */
+ * current device.  page_bytes (block_size * Hkv * dim * 2 in a 16-bit cache) must be a
+ * multiple of 4; pages of a multiple of 16 at 16-byte aligned bases move 16 bytes at a time,
+ * others (the scales of an 8-bit cache: Hkv * 4 bytes) 4 at a time.  Ids outside a pool are skipped and set B200_STATUS_BAD_BLOCK.  Bit-exact. */
 int b200_copy_blocks(const void* src_cache, void* dst_cache,
                      const int32_t* src_block_ids, const int32_t* dst_block_ids, int num_ids,
                      int64_t page_bytes, int num_src_blocks, int num_dst_blocks,

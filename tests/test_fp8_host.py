@@ -1,5 +1,6 @@
 """8-bit cache: what the host refuses (no GPU needed; nothing is launched), and the oracle's rounding."""
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -103,3 +104,58 @@ def test_prefill_refusals(lib, change, code):
     a.update(change)
     assert lib.b200_paged_prefill_gqa_fp8(*a.values()) == code
     assert b"paged_prefill_gqa_fp8" in lib.b200_last_error()
+
+
+def _model(**more):
+    cfg = SimpleNamespace(head_dim=128, num_layers=3, rms_eps=1e-6)
+    model = SimpleNamespace(cfg=cfg, n_q_local=8, n_kv_local=2, w={}, layer_prefix=lambda i: f"model.layers.{i}.",
+                            device="cpu", dtype=torch.bfloat16, ATTENTION_FAMILY="gqa", _gqa_b200_kv_dtype=E4M3)
+    model.__dict__.update(more)
+    return model
+
+
+def test_a_model_that_asks_for_8_bit_caches_gets_their_backend():
+    from auto_infer_b200 import gqa, registry
+    for mode, cls, base in (("paged", gqa.B200Fp8GqaBackend, gqa.B200GqaBackend),
+                            ("graph", gqa.B200GraphFp8GqaBackend, gqa.B200GraphGqaBackend)):
+        backend, caches = registry.build_attention_backend(_model(), mode, 5, 64)
+        assert type(backend) is cls and isinstance(backend, base) and len(caches) == 3
+        for k, v, ks, vs in caches:
+            assert k.shape == v.shape == (5, 64, 2, 128) and k.dtype == v.dtype == E4M3
+            assert ks.shape == vs.shape == (5, 2) and ks.dtype == vs.dtype == torch.float32
+            assert not ks.any() and not vs.any() and k.data_ptr() != v.data_ptr()
+        backend, caches = registry.build_mtp_attention_backend(_model(), mode, "model.mtp_layers.0.", 2, 16)
+        assert type(backend) is cls and backend.num_layers == 1 and len(caches) == 1
+        assert type(registry.build_attention_backend(_model(_gqa_b200_kv_dtype=torch.bfloat16), mode, 2, 16)[0]) is base
+    with pytest.raises(ValueError, match="unsupported _gqa_b200_kv_dtype"):
+        registry.build_attention_backend(_model(_gqa_b200_kv_dtype=torch.float16), "paged", 2, 16)
+    with pytest.raises(NotImplementedError):
+        registry.build_attention_backend(_model(), "dense")
+    with pytest.raises(NotImplementedError, match="heads of 128"):
+        registry.build_attention_backend(_model(cfg=SimpleNamespace(head_dim=64, num_layers=1, rms_eps=1e-6)), "paged", 2, 16)
+    for bs in (8, 24, 2048):
+        with pytest.raises(ValueError, match="power of two"):
+            registry.build_attention_backend(_model(), "paged", 2, bs)
+
+
+def test_prologue_without_a_cache_needs_somewhere_to_put_the_keys(lib):
+    from auto_infer_b200 import ops
+    x = torch.zeros(1, 2, 128, dtype=torch.bfloat16)
+    cs = torch.zeros(1, 1, 128, dtype=torch.bfloat16)
+    slots = torch.zeros(1, dtype=torch.int32)
+    for kc, vc, sl, want_k in ((None, None, None, False), (x, None, slots, True), (None, None, slots, True), (x, x, None, True)):
+        with pytest.raises(ValueError, match="go together"):
+            ops.gqa_rope_cache(x, x, x, cs, cs, kc, vc, sl, want_k=want_k)
+    a = dict(q=1 << 20, q_stride=256, k=1 << 20, k_stride=256, v=1 << 20, v_stride=256, cos=1 << 20, sin=1 << 20, cs=128,
+             qn=None, kn=None, eps=1e-6, q_out=1 << 20, q_out_stride=256, k_out=None, key_cache=None, value_cache=None,
+             slots=None, t=1, n_q=2, n_kv=2, d=128, block_size=0, num_blocks=0, status=None, stream=None)
+    for change in (dict(), dict(k_out=1 << 20, slots=1 << 20), dict(k_out=1 << 20, key_cache=1 << 20),
+                   dict(k_out=1 << 20, key_cache=1 << 20, value_cache=1 << 20, slots=1 << 20)):
+        assert lib.b200_gqa_rope_cache(*(a | change).values()) == -1
+
+
+def test_page_copy_refuses_what_is_not_words(lib):
+    a = dict(src=1 << 20, dst=1 << 21, src_ids=1 << 22, dst_ids=None, num_ids=2, page_bytes=12, src_blocks=4, dst_blocks=4,
+             status=None, stream=None)
+    for change in (dict(page_bytes=6), dict(src=(1 << 20) + 2), dict(dst=(1 << 21) + 1)):
+        assert lib.b200_copy_blocks(*(a | change).values()) == -3

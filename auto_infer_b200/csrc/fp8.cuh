@@ -46,6 +46,13 @@ __device__ __forceinline__ uint32_t f32x4_to_e4m3x4(float a, float b, float c, f
   return r;
 }
 
+// Two f16 to two codes (low half in the low byte), round to nearest even.
+__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(uint32_t h) {
+  uint16_t codes;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(codes) : "r"(h));
+  return codes;
+}
+
 // Smallest power of two s >= 2^-126 with a <= 448 * s, for a finite a >= 0.  448 = 1.75 * 2^8, so
 // with a = m * 2^e, 1 <= m < 2, the exponent is e - 8, or e - 7 when m > 1.75.
 __device__ __forceinline__ float fp8_scale_of(float a) {

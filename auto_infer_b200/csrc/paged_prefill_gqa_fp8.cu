@@ -23,13 +23,14 @@
 //   scales, or one pair for the whole tile when pages hold 128 tokens or more.
 //
 // Tensor-bound: flops = 4 * 128 * sum over rows of visible keys; 1024 tensor cycles and 1024 cycles of exponentials for a
-// tile of 128 x 128, while the whole tile takes about 2100: the chain scores -> maximum -> weights -> P V of the two
-// groups over one O.  Measured (one 8-kv-head GQA layer, 32 query heads): 581 us on an 8192-token prompt (945
-// TFLOP/s), 117 us on four 512-token chunks over cached prefixes, 50 us on 5-token drafts over 2 to 8 thousand
-// tokens.  What else was tried: both groups on row tiles of their own with one K / V stream (620 us: the instruction
-// footprint of two O rescales), the groups' exponential sections kept apart by a barrier (799 us against 742 at the time).
-// All roles' loops share the SM's instruction cache, so each piece of code is instantiated once and outer loops are not
-// unrolled: from 85 KB of code to 64 KB, with the waits in line, took 742 us to 581.
+// tile of 128 x 128.  A tile takes about 1850 cycles: each group's chain scores -> maximum -> weights -> P is about 3700
+// long, two of them run, and a softmax warp issues an instruction in about three cycles.  Where an item ends, O has
+// to be read before the next item's first P V.  Measured (32 query heads, 8 kv heads): 525 us on an 8192-token prompt (1046
+// TFLOP/s), 106 us on four 512-token chunks over cached prefixes, 41 us on 16 drafts of 5 tokens over 2 to 8
+// thousand tokens.  What else was tried: both groups on row tiles of their own with one K / V stream (620 us: the
+// instruction footprint of two O rescales), the groups' exponential sections kept apart by a barrier (799 us against 742 at
+// the time).  All roles' loops share the SM's instruction cache, so each piece of code is instantiated once and outer
+// loops are not unrolled: from 85 KB of code to 64 KB, with the waits in line, took 742 us to 581.
 #include "fp8.cuh"
 #include "prefill_plan.cuh"
 #include "tc05.cuh"
@@ -45,12 +46,12 @@ constexpr int kP8Groups = kPfTile / kFp8MinBlockSize;           // column groups
 constexpr int kP8SoftmaxThreads = 256;
 constexpr int kP8ConvertThreads = 128;
 constexpr int kP8Threads = kP8SoftmaxThreads + 128 + kP8ConvertThreads;   // whole warpgroups: 512 = 4 x 128
-// Registers per thread after the hand-over: 256 * 192 + 128 * 56 + 128 * 72 = 512 * 128.  Below 56 the producer and the
-// MMA issuers spill inside their loops, which is dear where shared memory leaves no L1 (200 / 40 / 72: 123 us instead of
-// 117 on four 512-token chunks); at 192 the softmax threads do not spill.
-constexpr int kP8RegsSoftmax = 192;
+// Registers per thread after the hand-over: 256 * 184 + 128 * 56 + 128 * 88 = 512 * 128.  Spills inside a loop are dear
+// where shared memory leaves little L1; with one page per tile there are none.  192 / 56 / 72 and 192 / 48 / 80: 117 and
+// 111 us instead of 106 on four 512-token chunks, and up to 4 % less on pages of 32 tokens.
+constexpr int kP8RegsSoftmax = 184;
 constexpr int kP8RegsOther = 56;
-constexpr int kP8RegsConvert = 72;
+constexpr int kP8RegsConvert = 88;
 constexpr int kP8TmemCols = 512;          // S0 [0,128) S1 [128,256) O [256,384) P_A [384,448) P_B [448,512)
 constexpr int kP8OCol = 256;
 constexpr int kP8PCol = 384;
@@ -116,26 +117,27 @@ struct Prefill8Params {
 __host__ __device__ constexpr uint32_t umma_idesc_type0(int m, int n, bool b_mn_major) {
   return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// Waits for a phase of an mbarrier, at most about two seconds: the unit suspends the thread for up to a millisecond
-// at a time.  Then the CTA's abort flag goes up: every later wait returns at once, so control flow stays uniform, the
-// kernel drains to its end and reports B200_STATUS_WAIT_TIMEOUT there.  A dozen instructions: it stands at every wait
-// of loops that together have to stay in the instruction cache.
+// Waits for a phase of an mbarrier, at most 2^20 tries of up to about 1.5 us each, which is how long the unit suspends a
+// thread by default (a longer hint wakes it later: 582 us instead of 568 on an 8192-token prompt).  Then the CTA's abort
+// flag goes up: every later wait returns at once, so control flow stays uniform, the kernel drains to its end and reports
+// B200_STATUS_WAIT_TIMEOUT there.  A dozen instructions: it stands at every wait of loops that together have to stay in the
+// instruction cache.
 __device__ __forceinline__ void mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t abort_at) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .u32 left, gone;\n\t"
-      "mov.u32 left, 2000;\n"
+      "mov.u32 left, 0x100000;\n"
       "again:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1, %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
       "@p bra through;\n\t"
-      "ld.volatile.shared.u32 gone, [%3];\n\t"
+      "ld.volatile.shared.u32 gone, [%2];\n\t"
       "setp.ne.u32 p, gone, 0;\n\t"
       "@p bra through;\n\t"
       "sub.u32 left, left, 1;\n\t"
       "setp.ne.u32 p, left, 0;\n\t"
       "@p bra again;\n\t"
-      "st.volatile.shared.u32 [%3], 1;\n"
+      "st.volatile.shared.u32 [%2], 1;\n"
       "through:\n\t}"
-      ::"r"(smem_u32(bar)), "r"(parity), "r"(1000000u), "r"(abort_at)
+      ::"r"(smem_u32(bar)), "r"(parity), "r"(abort_at)
       : "memory");
 }
 
@@ -262,9 +264,9 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         const int32_t* const table = p.block_table + (int64_t)item.seq * p.bt_stride;
         const int last_block = (item.kv_len - 1) >> p.block_shift;
         const int cols = item.seq < p.table_rows ? p.table_cols : 0;
-        // The next item is drawn four tiles before this one's last load: the convert warps stage its Q
+        // The next item is drawn eight tiles before this one's last load: the convert warps stage its Q
         // while this item's last tiles are worked on.
-        const int draw_at = n > 4 ? n - 4 : 0;
+        const int draw_at = n > 8 ? n - 8 : 0;
         // K and V travel through separate rings (a K stage is free again as soon as S = Q K^T has run), the K loads
         // kP8KLead tiles ahead of the V loads, which take the page ids from the K loads' look-up.
         int ids[kP8KLead + 1];                       // of tiles step, step - 1, ..: lane g < 8 has the page of column group g
@@ -426,7 +428,9 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       if (take_item(item_no, item) < 0) break;
       const int rg = item.row0 + r;
       const bool valid = rg < item.q_len * G;
-      const int lim = valid ? min(item.causal_base + rg / G, item.kv_len - 1) : -1;
+      // rows past the item's see whatever there is: nobody reads their O
+      const int lim = valid ? min(item.causal_base + rg / G, item.kv_len - 1) : INT_MAX;
+      const bool idle = !__any_sync(0xffffffffu, valid);
       mbar_wait_limited(&sm.q_full[item_no & 1u], (item_no >> 1) & 1u, abort_at);
       const float row_factor = sm.row_factor[item_no & 1u][r];
       float m = -INFINITY;           // running maximum of this group's scores: what its row sum is scaled to
@@ -438,6 +442,36 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         const uint32_t s_col = lane_base + sb * 128;
         constexpr int kN = kOnePage ? 1 : kP8Groups;   // pairs of scales of a tile
         const uint32_t sl = it % kP8ScaleSlots;
+        mbar_wait_limited(&sm.s_full[sb], (it >> 1) & 1u, abort_at);
+        tc_fence_after();
+        if (idle) {                                    // no row of this warp counts: keep the barriers going
+          mbar_arrive(&sm.s_empty[sb]);
+          // a phase of m_ready may not get this warp's arrivals of two tiles: the group is through with its previous one
+          if (it >= 2) mbar_wait_limited(&sm.p_full[g], ((it - 2) >> 1) & 1u, abort_at);
+          mbar_arrive(&sm.m_ready[it & 1u]);
+          mbar_arrive(&sm.p_full[g]);
+          continue;
+        }
+        // Columns past the row's limit become -inf in place, a quarter of the row at a time: few tiles need it, and code
+        // that runs rarely is fetched from far away each time (unrolled over the row it cost 3000 cycles a tile).
+        const int last_col = lim - tile * kPfTile;
+        if (__builtin_expect(__any_sync(0xffffffffu, last_col < kPfTile - 1), 0)) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < kPfTile; c0 += 32) {
+            uint32_t x[32];
+            tmem_ld32(s_col + c0, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = c0 + c > last_col ? 0xff800000u : x[c];
+            tmem_st32(s_col + c0, x);
+          }
+          tmem_wait_st();
+        }
+        // The whole score row goes to registers in one go and the S buffer straight back to
+        // the MMA issuer.
+        uint32_t sv[4][32];
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) tmem_ld32(s_col + q4 * 32, sv[q4]);
         mbar_wait_limited(&sm.scale_full[sl], (it / kP8ScaleSlots) & 1u, abort_at);
         float f[kN], lv[kN];                           // product -> log2 score; log2 of V's scale
 #pragma unroll
@@ -447,25 +481,15 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           f[i] = f[i] < 1.17549435e-38f ? 1.17549435e-38f : f[i];
           lv[i] = fast_log2(sm.tile_scale[sl][1][i]);
         }
-        mbar_wait_limited(&sm.s_full[sb], (it >> 1) & 1u, abort_at);
-        tc_fence_after();
-        const int tbase = tile * kPfTile;
-        const bool need_mask = tbase + kPfTile - 1 > lim;
-        // The whole score row goes to registers in one go and the S buffer straight back to
-        // the MMA issuer.
-        uint32_t sv[4][32];
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) tmem_ld32(s_col + q4 * 32, sv[q4]);
+        // the reference O is scaled to after the previous tile (owned by the other group)
+        float m_in = -INFINITY;
+        if (tile > 0) {
+          mbar_wait_limited(&sm.m_ready[(it - 1) & 1u], ((it - 1) >> 1) & 1u, abort_at);
+          m_in = sm.row_ms[(it - 1) & 1u][r];
+        }
         tmem_wait_ld();
         tc_fence_before();
         mbar_arrive(&sm.s_empty[sb]);
-        if (__builtin_expect(need_mask, 0)) {
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4)
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (tbase + q4 * 32 + c > lim) sv[q4][c] = __float_as_uint(-INFINITY);
-        }
         // maximum of the scores, and of the scores plus log2 of V's scale
         float mx = -INFINITY, my = -INFINITY;
         {
@@ -490,12 +514,6 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
               my = fmaxf(my, x + lv[u]);
             }
           }
-        }
-        // the reference O is scaled to after the previous tile (owned by the other group)
-        float m_in = -INFINITY;
-        if (tile > 0) {
-          mbar_wait_limited(&sm.m_ready[(it - 1) & 1u], ((it - 1) >> 1) & 1u, abort_at);
-          m_in = sm.row_ms[(it - 1) & 1u][r];
         }
         // lazy rescale: only when some row of the warp outgrew the stale reference by 2^8
         const bool grow = my - m_in > 8.f || (m_in == -INFINITY && my > -INFINITY);
@@ -594,69 +612,89 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     }
   } else {
     // ------------------- convert: Q terms, V to f16, epilogue -------------------
-    // Thread e owns query row e: it stages the row's two e4m3 terms two tiles before the previous
-    // item ends, and takes row e of O out of tensor memory at the end.  In between the 128 threads turn
-    // each V tile's codes into f16, one tile ahead of its P V or more.
+    // Thread e owns query row e: it stages the row's two e4m3 terms while the item before is worked on, and takes row e
+    // of O out of tensor memory at the end.  In between the 128 threads turn each V tile's codes into f16, one tile
+    // ahead of its P V or more.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kP8RegsConvert));
     const int r = threadIdx.x - (kP8Threads - kP8ConvertThreads);
     const uint32_t o_col = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kP8OCol;
     const int G = p.group;
     uint32_t it = 0;                                 // next V tile to convert, over all items
-    auto rows_of = [&](const PrefillItem& x) -> int {
-      return x.q_start + x.q_len <= p.num_tokens ? x.q_len * G : 0;
+    // Q of the next item: thread e quantises row e.  Its largest magnitude is looked for first, then eight steps convert 16
+    // elements each behind the item's last V tiles; what a step loads arrives while a tile is converted.  (All at once
+    // before the last V tile it took 10000 cycles, and that tile's P V and the next item's first S waited for it.)
+    constexpr int kSteps = 8;
+    const uint4* q_row = nullptr;                    // null: a row past the item's, zeros
+    int step = kSteps;                               // next step of the item; kSteps: none
+    float up = 0.f, row_factor = 0.f;
+    uint4 raw[2];
+    auto load_step = [&]() {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) raw[i] = q_row ? q_row[2 * step + i] : make_uint4(0u, 0u, 0u, 0u);
     };
-    auto stage_q = [&](const PrefillItem& x, uint32_t k) {
+    struct Row {                                     // what this thread keeps of an item
+      int n_tiles, kv_len;
+      int64_t out;                                   // its row e among the rows of `out`, or -1
+    };
+    auto begin_q = [&](const PrefillItem& x) -> Row {
+      const bool fits = x.q_start + x.q_len <= p.num_tokens;
       const int rg = x.row0 + r;
-      const bool valid = rg < rows_of(x);
-      if (r == 0 && rows_of(x) < x.q_len * G && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(valid ? x.q_start + rg / G : 0) * p.q_stride +
-                                                        (int64_t)(valid ? x.kv_head * G + rg % G : 0) * kPfHeadDim);
-      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-      uint32_t top = 0;
+      if (r == 0 && !fits && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
+      const bool valid = fits && rg < x.q_len * G;
+      const int64_t tok = x.q_start + rg / G;
+      const int head = x.kv_head * G + rg % G;
+      q_row = valid ? reinterpret_cast<const uint4*>(p.q + tok * p.q_stride + (int64_t)head * kPfHeadDim) : nullptr;
+      step = 0;
+      uint32_t top = 0;                              // maxima of the even and the odd elements
 #pragma unroll 1
-      for (int c0 = 0; c0 < 16; c0 += 8) {
+      for (int c0 = 0; c0 < 16 && valid; c0 += 8) {
         uint4 v[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = valid ? src[c0 + c] : zero;
+        for (int c = 0; c < 8; ++c) v[c] = q_row[c0 + c];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+          const uint32_t a = __vmaxu2(v[c].x & 0x7fff7fffu, v[c].y & 0x7fff7fffu);
+          const uint32_t b = __vmaxu2(v[c].z & 0x7fff7fffu, v[c].w & 0x7fff7fffu);
+          top = __vmaxu2(top, __vmaxu2(a, b));
         }
       }
-      const int e = max((int)(top >> 7), 8);                       // exponent field; 8 and more: both factors are normal
-      const float up = __uint_as_float((uint32_t)(261 - e) << 23); // 2^(7 - (e - 127))
-      mbar_wait_limited(&sm.q_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_at);
-      uint8_t* const hi_at = sm.q[k & 1u][0];
-      uint8_t* const lo_at = sm.q[k & 1u][1];
-#pragma unroll 1
-      for (int c = 0; c < 8; ++c) {                                // 16 dims at a time
-        const uint4 a = valid ? src[2 * c] : zero, b = valid ? src[2 * c + 1] : zero;
-        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x[4];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            x[2 * j] = __uint_as_float(w[2 * i + j] << 16) * up;
-            x[2 * j + 1] = __uint_as_float(w[2 * i + j] & 0xffff0000u) * up;
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = fmaf(x[j], 0.f, x[j]);  // infinities become NaN, which has a code
-          hi[i] = f32x4_to_e4m3x4(x[0], x[1], x[2], x[3]);
-          const uint32_t h0 = e4m3x2_to_f16x2((uint16_t)hi[i]), h1 = e4m3x2_to_f16x2((uint16_t)(hi[i] >> 16));
-          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-          const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-          lo[i] = f32x4_to_e4m3x4(x[0] - f0.x, x[1] - f0.y, x[2] - f1.x, x[3] - f1.y);
-        }
-        *reinterpret_cast<uint4*>(hi_at + swz128(r, c)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(lo_at + swz128(r, c)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      // exponent field of the largest; 8 and more: both factors are normal
+      const int e = max((int)(max(top & 0xffffu, top >> 16) >> 7), 8);
+      up = e == 255 ? NAN : __uint_as_float((uint32_t)(261 - e) << 23);   // 2^(7 - (e - 127)); any inf or NaN: the row is NaN
+      row_factor = __uint_as_float((uint32_t)(e - 7) << 23) * p.scale_log2;
+      return Row{x.n_tiles, x.kv_len, valid ? tok * p.num_q_heads + head : -1};
+    };
+    auto put_step = [&](uint32_t k) {
+      if (step == 0) {
+        // the buffers' last reader is the item two before: its S has run, its softmax (the epilogue waited for it) is over
+        mbar_wait_limited(&sm.q_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_at);
+        sm.row_factor[k & 1u][r] = row_factor;
       }
-      sm.row_factor[k & 1u][r] = __uint_as_float((uint32_t)(e - 7) << 23) * p.scale_log2;
-      fence_proxy_async_smem();
-      mbar_arrive(&sm.q_full[k & 1u]);
+      const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        uint32_t h[2], l[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          // f16 holds what e4m3 can: elements under 2^-14 here are rounded to 0 by either
+          const uint32_t x = pack_f16(__uint_as_float(w[i + j] << 16) * up, __uint_as_float(w[i + j] & 0xffff0000u) * up);
+          h[j] = f16x2_to_e4m3x2(x);
+          const uint32_t back = e4m3x2_to_f16x2((uint16_t)h[j]);
+          const __half2 rest = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&back));
+          l[j] = f16x2_to_e4m3x2(*reinterpret_cast<const uint32_t*>(&rest));
+        }
+        hi[i >> 1] = __byte_perm(h[0], h[1], 0x5410);
+        lo[i >> 1] = __byte_perm(l[0], l[1], 0x5410);
+      }
+      const uint32_t at = swz128(r, step);
+      *reinterpret_cast<uint4*>(sm.q[k & 1u][0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(sm.q[k & 1u][1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (step == kSteps - 1) {
+        fence_proxy_async_smem();
+        mbar_arrive(&sm.q_full[k & 1u]);
+      }
+      ++step;
     };
     // Bank conflicts: the eight lanes of a phase read and write 16-byte chunks of two rows, four chunks (half a row of
     // codes) each.  Under the 128-byte swizzle a row's chunk number is XOR-ed with row & 7; rows whose numbers
@@ -664,17 +702,20 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     // the other (bit 2); writing 16 codes as two chunks of f16, even chunks of one row and odd ones of the other (bit 0).
     const int pair = lane >> 3;                                    // rows {0,5}, {1,4}, {2,7}, {3,6} of each eight
     const int row0 = (warp & 3) * 32 + (lane & 4 ? pair ^ 5 : pair);
-    auto convert = [&](const PrefillItem& x, int step) {
-      const int have = x.kv_len - step * kPfTile;                  // rows past the end are zero: 0 x NaN is NaN
+    // rows row0 + 8 i share row & 7: i is a constant offset, the other chunks are XORs of a constant
+    const uint32_t rd_at = swz128(row0, lane & 3), wr_at = swz128(row0, 2 * (lane & 3));
+    auto convert = [&](int kv_len, int step) {
+      const int have = kv_len - step * kPfTile;                  // rows past the end are zero: 0 x NaN is NaN
       const int sv = it % kP8VStages, b = it & 1u;
       mbar_wait_limited(&sm.v_full[sv], (it / kP8VStages) & 1u, abort_at);
       if (it >= 2) mbar_wait_limited(&sm.pv_done[b], ((it - 2) >> 1) & 1u, abort_at);
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         uint4 v[4];
+        const uint8_t* const src = sm.v[sv] + (rd_at ^ (uint32_t)(64 * half));
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          v[i] = *reinterpret_cast<const uint4*>(sm.v[sv] + swz128(row0 + 8 * i, half * 4 + (lane & 3)));
+          v[i] = *reinterpret_cast<const uint4*>(src + 1024 * i);
         if (have < kPfTile) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -686,7 +727,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            *reinterpret_cast<uint4*>(dst + swz128(row0 + 8 * i, 2 * (lane & 3) + j)) =
+            *reinterpret_cast<uint4*>(dst + (wr_at ^ (uint32_t)(16 * j)) + 1024 * i) =
                 make_uint4(e4m3x2_to_f16x2((uint16_t)w[2 * j]), e4m3x2_to_f16x2((uint16_t)(w[2 * j] >> 16)),
                            e4m3x2_to_f16x2((uint16_t)w[2 * j + 1]), e4m3x2_to_f16x2((uint16_t)(w[2 * j + 1] >> 16)));
         }
@@ -697,28 +738,30 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       ++it;
     };
     // One instance of each piece of code (see the producer): iteration k works on item k - 1, whose Q was staged in the
-    // iteration before; it stages item k before its own last V tile and writes item k - 2 behind its first.
-    PrefillItem item{}, prev{}, next{};
+    // iteration before; it stages item k behind its own last V tiles and writes item k - 2 behind its first.
+    Row item{}, prev{}, next{};
     int total = -1;                                  // items of this CTA, once known
 #pragma unroll 1
     for (int k = 0; total < 0 || k < total + 2; ++k) {
       const int n = item.n_tiles;
+      const int take_at = n > kSteps + 1 ? n - kSteps - 1 : 0;
 #pragma unroll 1
-      for (int tile = 0; tile == 0 || tile < n; ++tile) {
-        if (total < 0 && tile >= n - 1) {
-          if (take_item(k, next) >= 0)
-            stage_q(next, k);
+      for (int tile = 0; tile == 0 || tile < n || step < kSteps; ++tile) {
+        if (total < 0 && tile == take_at) {
+          PrefillItem rec;
+          if (take_item(k, rec) >= 0)
+            next = begin_q(rec);
           else
             total = k;
         }
-        if (n > 0) convert(item, tile);
+        const bool stage = step < kSteps && (tile > 0 || k < 2);
+        if (stage) load_step();
+        if (tile < n) convert(item.kv_len, tile);
+        if (stage) put_step(k);
         if (tile > 0 || k < 2) continue;
         const uint32_t item_no = k - 2;
         // ---- epilogue: row e of O out of tensor memory as soon as the item's last P V has run
-        const int rg = prev.row0 + r;
-        const bool valid = rg < rows_of(prev);
-        const int64_t tok = prev.q_start + (valid ? rg / G : 0);
-        const int head = prev.kv_head * G + (valid ? rg % G : 0);
+        const bool valid = prev.out >= 0;
         mbar_wait_limited(&sm.l_full, item_no & 1u, abort_at);
         const float m0 = sm.row_m[0][r], m1 = sm.row_m[1][r], mo = sm.row_mfin[r];
         const float mm = fmaxf(m0, m1);
@@ -745,9 +788,18 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             mbar_arrive(&sm.o_free);
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = empty ? 0u : __float_as_uint(__uint_as_float(o[i]) * half_unit * inv);
+          for (int i = 0; i < 32; i += 2) {
+            float2 x = __fmul2_rn(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(half_unit, half_unit));
+            x = __fmul2_rn(x, make_float2(inv, inv));
+            o[i] = __float_as_uint(x.x);
+            o[i + 1] = __float_as_uint(x.y);
+          }
+          if (empty) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
           if (valid) {
-            const int64_t off = (tok * p.num_q_heads + head) * kPfHeadDim + q4 * 32;
+            const int64_t off = prev.out * kPfHeadDim + q4 * 32;
             if (p.out_is_f32) {
               float* dst = reinterpret_cast<float*>(p.out) + off;
 #pragma unroll
@@ -768,7 +820,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           }
         }
         if (valid && p.lse_out)
-          p.lse_out[tok * p.num_q_heads + head] = empty ? -INFINITY : mm * 0.6931471805599453f + __logf(lsum);
+          p.lse_out[prev.out] = empty ? -INFINITY : mm * 0.6931471805599453f + __logf(lsum);
       }
       prev = item;
       item = next;

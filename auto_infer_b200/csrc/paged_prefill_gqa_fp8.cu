@@ -46,12 +46,15 @@ constexpr int kP8Groups = kPfTile / kFp8MinBlockSize;           // column groups
 constexpr int kP8SoftmaxThreads = 256;
 constexpr int kP8ConvertThreads = 128;
 constexpr int kP8Threads = kP8SoftmaxThreads + 128 + kP8ConvertThreads;   // whole warpgroups: 512 = 4 x 128
-// Registers per thread after the hand-over: 256 * 184 + 128 * 56 + 128 * 88 = 512 * 128.  Spills inside a loop are dear
-// where shared memory leaves little L1; with one page per tile there are none.  192 / 56 / 72 and 192 / 48 / 80: 117 and
-// 111 us instead of 106 on four 512-token chunks, and up to 4 % less on pages of 32 tokens.
-constexpr int kP8RegsSoftmax = 184;
-constexpr int kP8RegsOther = 56;
-constexpr int kP8RegsConvert = 88;
+// Registers per thread after the hand-over, softmax, producer and issuers, convert: 256 * 184 + 128 * 56 + 128 * 88 =
+// 256 * 192 + 128 * 48 + 128 * 80 = 512 * 128.  Spills inside a loop are dear where shared memory leaves little L1.
+// With one page per tile the first split has none (106 us on four 512-token chunks, 111 with the second); the eight
+// pairs of scales of smaller pages need the second's softmax registers (97 us on three sequences over pages of 32 tokens,
+// 103 with the first).
+template <bool kOnePage>
+struct P8Regs {
+  static constexpr int kSoftmax = kOnePage ? 184 : 192, kOther = kOnePage ? 56 : 48, kConvert = kOnePage ? 88 : 80;
+};
 constexpr int kP8TmemCols = 512;          // S0 [0,128) S1 [128,256) O [256,384) P_A [384,448) P_B [448,512)
 constexpr int kP8OCol = 256;
 constexpr int kP8PCol = 384;
@@ -225,7 +228,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
   };
 
   if (warp >= 8 && warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kP8RegsOther));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P8Regs<kOnePage>::kOther));
     if (warp == 8) {
       // ------------------------------ TMA producer ------------------------------
       if (lane == 0) {
@@ -413,7 +416,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       __syncwarp();
     }
   } else if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kP8RegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P8Regs<kOnePage>::kSoftmax));
     // -------------------------------- softmax --------------------------------
     const int g = warp >> 2;                         // group: KV tiles whose running index & 1 == g
     const int r = threadIdx.x & 127;                 // query row of the tile == TMEM lane
@@ -615,7 +618,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     // Thread e owns query row e: it stages the row's two e4m3 terms while the item before is worked on, and takes row e
     // of O out of tensor memory at the end.  In between the 128 threads turn each V tile's codes into f16, one tile
     // ahead of its P V or more.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kP8RegsConvert));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P8Regs<kOnePage>::kConvert));
     const int r = threadIdx.x - (kP8Threads - kP8ConvertThreads);
     const uint32_t o_col = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kP8OCol;
     const int G = p.group;

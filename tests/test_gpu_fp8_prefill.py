@@ -301,3 +301,29 @@ def test_refusals():
 def _b200_error():
     from auto_infer_b200._lib import B200Error
     return B200Error
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_query_that_is_not_finite_spoils_its_own_row_only(bad):
+    c = list(_case(31, [300, 40], [45, 40], 8, 2, 32))
+    c[0][[3, 60], [1, 7], [0, 127]] = bad
+    got, lse = _run(*c)
+    spoilt = torch.zeros(got.shape[:2], dtype=torch.bool)
+    spoilt[[3, 60], [1, 7]] = True
+    assert got[spoilt].isnan().all()
+    clean = c[0].clone()
+    clean[spoilt] = 0
+    want, want_lse = _run(clean, *c[1:])
+    assert torch.equal(got[~spoilt], want[~spoilt]) and torch.equal(lse[~spoilt], want_lse[~spoilt])
+
+
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 64, 96, 127])
+def test_warps_without_rows(rows):
+    """Items whose last rows are missing, over an odd and an even number of tiles, before and after full ones on one CTA."""
+    lens, q_lens = [700, 128 + rows, 140, 513, rows], [rows, 128, 3, rows, rows]
+    for bs in (32, 128):
+        c = _case(rows, lens, q_lens, 1, 1, bs)
+        first, lse = _run(*c)
+        _check(first, lse, *c)
+        again, lse2 = _run(*c, max_ctas=1)
+        assert torch.equal(first, again) and torch.equal(lse, lse2)

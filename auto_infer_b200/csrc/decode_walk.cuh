@@ -64,7 +64,7 @@ __device__ __forceinline__ void merge_noted_pairs(const Params& p, const int* li
       acc[0] += wgt * a.x; acc[1] += wgt * a.y; acc[2] += wgt * a.z; acc[3] += wgt * a.w;
       acc[4] += wgt * b.x; acc[5] += wgt * b.y; acc[6] += wgt * b.z; acc[7] += wgt * b.w;
     }
-    const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+    const float inv = wsum == 0.f ? 0.f : 1.f / wsum;        // a NaN sum (8-bit cache: a NaN lse) stays one
     const int64_t tok = q_start + row / G;
     const int head = kv_head * G + row % G;
     const int64_t off = (tok * p.num_q_heads + head) * kHeadDim + col;
@@ -79,7 +79,7 @@ __device__ __forceinline__ void merge_noted_pairs(const Params& p, const int* li
       *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.out) + off) = pk;
     }
     if (p.lse_out && (t & 15) == 0)
-      p.lse_out[tok * p.num_q_heads + head] = wsum > 0.f ? mx + __logf(wsum) : -INFINITY;
+      p.lse_out[tok * p.num_q_heads + head] = wsum == 0.f ? -INFINITY : mx + __logf(wsum);
   }
 }
 #endif  // __CUDACC__

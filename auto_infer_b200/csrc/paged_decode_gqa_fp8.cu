@@ -489,7 +489,8 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int ex = max((int)(top >> 7), 15);                     // exponent field; at least 15 keeps both factors normal
-        const float up = __uint_as_float((uint32_t)(268 - ex) << 23); // 2^(14 - (ex - 127))
+        // 2^(14 - (ex - 127)); any infinity or NaN makes the row NaN, also where all its scores would be -inf
+        const float up = ex == 255 ? NAN : __uint_as_float((uint32_t)(268 - ex) << 23);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const uint2 v = qraw[n][ks];
@@ -676,9 +677,9 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       }
       // O is in units of 2^go, the sum in units of 2^g; the factor between them in two halves, each of
       // which fp32 holds however far apart they are
-      inv_r[h] = lsum > 0.f ? 1.f / lsum : 0.f;
+      inv_r[h] = lsum == 0.f ? 0.f : 1.f / lsum;          // a NaN sum stays one
       unit_r[h] = go == -INFINITY ? 0.f : fast_exp2((go - g) * 0.5f);
-      lse_r[h] = lsum > 0.f ? g * 0.6931471805599453f + __logf(lsum) : -INFINITY;
+      lse_r[h] = lsum == 0.f ? -INFINITY : g * 0.6931471805599453f + __logf(lsum);
     }
     named_bar_sync(1, kF8Consumers);                           // (3) the four slots hold the warp-pair sums
     const bool record_fits = (item.direct || item.partial_idx < p.max_partials) && rows > 0;

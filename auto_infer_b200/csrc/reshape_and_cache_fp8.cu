@@ -112,13 +112,13 @@ __device__ __forceinline__ uint2 rescale8(const uint2& c, float ratio) {
 // A page's new scale: what the call asks for when the page starts anew, else the larger of that and the old one.
 struct PageScale {
   float s, inv;                // inv: 1 / s if that is exact and all elements are finite, else 0
-  float ratio;                 // what the page's other rows are multiplied by, 0 when they stay
+  float ratio;                 // what the page's other rows are multiplied by (0: too small for fp32), -1 when they stay
   __device__ __forceinline__ PageScale(uint32_t top, float s_old, bool first_row_written, bool all_finite) {
     const float s_call = fp8_scale_of(__uint_as_float(top << 16));
     const bool anew = first_row_written || !(s_old > 0.f && s_old < INFINITY);
     s = anew ? s_call : fmaxf(s_old, s_call);
     inv = all_finite && (__float_as_uint(s) & 0x7fffffu) == 0 ? 1.f / s : 0.f;
-    ratio = !anew && s > s_old ? s_old / s : 0.f;
+    ratio = !anew && s > s_old ? s_old / s : -1.f;
   }
 };
 __device__ __forceinline__ uint32_t larger_half(uint32_t top) { return max(top & 0xffffu, top >> 16); }
@@ -272,7 +272,7 @@ reshape_and_cache_fp8_kernel(const QuantWriteParams p) {
                   quantise8_any(*reinterpret_cast<const uint4*>(src + (int64_t)at.x * stride), ps.s);
           }
         }
-        if (ps.ratio != 0.f)                       // a grown scale: round the page's other rows to it
+        if (ps.ratio >= 0.f)                       // a grown scale: round the page's other rows to it
 #pragma unroll 1
           for (int r = half; r < p.block_size; r += 2)
             if (token_of[r] < 0) {
@@ -355,7 +355,7 @@ reshape_and_cache_fp8_kernel(const QuantWriteParams p) {
               *reinterpret_cast<uint2*>(rows_at + r * row_bytes) =
                   quantise8_any(*reinterpret_cast<const uint4*>(src + (int64_t)token_of[r] * stride), ps.s);
         }
-        if (ps.ratio != 0.f)
+        if (ps.ratio >= 0.f)
 #pragma unroll 1
           for (int r = first; r < p.block_size; r += kStep)
             if (token_of[r] < 0) {

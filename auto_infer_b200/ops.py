@@ -181,6 +181,11 @@ def _device_of(first, *others) -> int:
     return index
 
 
+def _as_int32(ids: torch.Tensor) -> torch.Tensor:
+    """Slots or block ids in 32 bits; what does not fit stays out of range."""
+    return ids if ids.dtype is _I32 else ids.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+
+
 def _aligned_rows(x: torch.Tensor, row: int) -> torch.Tensor:
     """``x`` (T, heads, D) with its heads contiguous, tokens a multiple of 16 bytes apart and a
     16-byte aligned base: itself when it is so already, else a copy."""
@@ -210,8 +215,7 @@ def reshape_and_cache_fp8(key: torch.Tensor, value: torch.Tensor, key_cache: tor
     if t == 0:
         return
     key, value = _aligned_rows(key, n_kv * d), _aligned_rows(value, n_kv * d)
-    if slot_mapping.dtype is not _I32 or not slot_mapping.is_contiguous():
-        slot_mapping = slot_mapping.to(torch.int32).contiguous()
+    slot_mapping = _as_int32(slot_mapping).contiguous()
     _call_on(index, "b200_reshape_and_cache_fp8", key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0),
              key_cache.data_ptr(), value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(),
              slot_mapping.data_ptr(), t, n_kv, d, block_size, num_blocks)
@@ -409,10 +413,12 @@ def paged_decode_gqa_write(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Te
     return out
 
 
-def _fp8_attention_args(who, q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
+def _fp8_attention_args(who, kind, q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
                         lse_out):
     """Checks and tensors shared by the attention calls over an 8-bit cache:
     (device index, q, block_table, out, cache shape)."""
+    if type(plan) is not kind:
+        raise ValueError(f"{who}: the plan must be a {kind.__name__}")
     index = _device_of(q, key_cache, value_cache, key_scale, value_scale, block_table, plan.dev, out, lse_out)
     shape = _check_fp8_cache(key_cache, value_cache, key_scale, value_scale)
     _, block_size, n_kv, d = shape
@@ -429,8 +435,7 @@ def _fp8_attention_args(who, q, key_cache, value_cache, key_scale, value_scale, 
     if len(table_shape) != 2 or table_shape[0] < plan.num_seqs or table_shape[1] * block_size < plan.max_kv:
         raise ValueError(f"{who}: block_table must have {plan.num_seqs} rows of at least "
                          f"{-(-plan.max_kv // block_size)} blocks")
-    if block_table.dtype is not _I32:
-        block_table = block_table.to(torch.int32)
+    block_table = _as_int32(block_table)
     if 0 in table_shape:                             # no sequence has keys: a table to point at, never read
         block_table = torch.zeros(1, 1, dtype=torch.int32, device=q.device)
     elif block_table.stride(1) != 1:
@@ -452,7 +457,7 @@ def paged_decode_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     """``paged_decode_gqa`` over an 8-bit cache (see ``reshape_and_cache_fp8``): the same plans, masks
     and outputs.  Rows of sequences the plan skipped are left untouched in ``out``."""
     index, q, block_table, out, (num_blocks, block_size, n_kv, d) = _fp8_attention_args(
-        "paged_decode_gqa_fp8", q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
+        "paged_decode_gqa_fp8", DecodePlan, q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
         lse_out)
     t, n_q, _ = q.shape
     rows, cols = block_table.shape
@@ -667,7 +672,7 @@ def paged_prefill_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache:
     """``paged_prefill_gqa`` over an 8-bit cache (see ``reshape_and_cache_fp8``): the same plans, masks
     and outputs.  Rows of sequences that are not in the plan are left untouched in ``out``."""
     index, q, block_table, out, (num_blocks, block_size, n_kv, d) = _fp8_attention_args(
-        "paged_prefill_gqa_fp8", q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
+        "paged_prefill_gqa_fp8", PrefillPlan, q, key_cache, value_cache, key_scale, value_scale, block_table, plan, out, out_f32,
         lse_out)
     t, n_q, _ = q.shape
     rows, cols = block_table.shape
@@ -832,8 +837,8 @@ def copy_blocks(source_caches, target_caches, block_ids, target_block_ids=None) 
                 target.shape[:block_axis] + target.shape[block_axis + 1:])
             if not same:
                 raise ValueError("source and target cache shapes must match")
-            if source.dtype != target.dtype:
-                raise ValueError("source and target cache types must match")
+            if source.element_size() != target.element_size():
+                raise ValueError("source and target cache types must match in size")
             _need_cuda(source, target)
             if not (source.is_contiguous() and target.is_contiguous()):
                 raise ValueError("caches must be contiguous")

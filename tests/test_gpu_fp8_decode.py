@@ -287,3 +287,33 @@ def test_refusals():
         ops.paged_decode_gqa_fp8(**{**good, "block_table": table.cpu()})
     empty = ops.DecodePlan([], [], 8, 2, "cuda")
     assert ops.paged_decode_gqa_fp8(**{**good, "plan": empty, "q": q[:0], "block_table": table[:0]}).shape == (0, 8, 128)
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("num_ctas", [1, 148])
+def test_a_query_that_is_not_finite_spoils_its_own_row_only(bad, num_ctas):
+    """Also where it makes every score -inf, and where its keys are cut across CTAs; a NaN key is no empty row either."""
+    c = list(_case(31, [3000, 40], [2, 1], 8, 2, 32))
+    c[0][[1, 2], [5, 0], [0, 127]] = bad
+    spoilt = torch.zeros(c[0].shape[:2], dtype=torch.bool)
+    spoilt[[1, 2], [5, 0]] = True
+    c[1][:, :, :, 0] = torch.tensor(1.0).to(c[1].dtype)      # the scores against the bad element all have one sign
+    got, lse = _run(*c, num_ctas=num_ctas)
+    assert got[spoilt].isnan().all() and lse[spoilt].isnan().all()
+    clean = c[0].clone()
+    clean[spoilt] = 0
+    want, want_lse = _run(clean, *c[1:], num_ctas=num_ctas)
+    assert torch.equal(got[~spoilt], want[~spoilt]) and torch.equal(lse[~spoilt], want_lse[~spoilt])
+
+
+def test_plans_of_another_kind_are_refused():
+    from auto_infer_b200 import ops
+    c = _case(32, [100, 50], [1, 30], 8, 2, 16)
+    dev = [x.cuda() for x in c[:6]]
+    decode = ops.DecodePlan(c[6], c[7], 8, 2, "cuda", capacity_seqs=2)
+    prefill = ops.PrefillPlan(c[6], c[7], 8, 2, "cuda", capacity_tokens=31, capacity_seqs=2)
+    latent = ops.MlaDecodePlan([1], [50], 2, "cuda")
+    for call, plans in ((ops.paged_decode_gqa_fp8, (prefill, latent)), (ops.paged_prefill_gqa_fp8, (decode, latent))):
+        for plan in plans:
+            with pytest.raises(ValueError, match="the plan must be"):
+                call(*dev, plan, c[8])

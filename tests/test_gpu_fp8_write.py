@@ -199,3 +199,30 @@ def test_refusals():
             ops.reshape_and_cache_fp8(**{**good, **change})
     with pytest.raises(RuntimeError):
         ops.reshape_and_cache_fp8(**{**good, "key": rows.cpu()})
+
+
+@pytest.mark.parametrize("old_rows, new_rows", [(1, [50]), (40, [50]), (40, list(range(41, 64)))])
+def test_a_scale_that_grows_further_than_a_quotient_can_say(old_rows, new_rows):
+    """Rows near the smallest normal numbers, then one near the largest: s_old / s is below what fp32 holds, and the
+    old rows become zeros rather than keep codes that now mean something else."""
+    g = torch.Generator().manual_seed(9)
+    kc, ks = empty_pool(2, 64, 2)
+    vc, vs = empty_pool(2, 64, 2)
+    tiny = _rows(g, old_rows, 2) * 2.0 ** -124
+    first = _check(tiny, tiny, kc, vc, ks, vs, list(range(old_rows)))
+    assert first[0].float()[0, :old_rows].abs().sum() > 0
+    huge = _rows(g, len(new_rows), 2) * 2.0 ** 100
+    got = _check(huge, huge, *first, new_rows)
+    assert (as_values(got[0])[0, :old_rows] == 0).all()
+
+
+def test_slots_of_64_bits_do_not_wrap_into_the_pool():
+    from auto_infer_b200 import ops
+    g = torch.Generator().manual_seed(10)
+    pool = [x.cuda() for x in (*empty_pool(2, 16, 1), *empty_pool(2, 16, 1))]
+    kc, ks, vc, vs = pool
+    rows = _rows(g, 3, 1).cuda()
+    ops.reshape_and_cache_fp8(rows, rows, kc, vc, ks, vs, torch.tensor([2 ** 32 + 5, -2 ** 32 + 6, 7]).cuda())
+    assert ops.read_status("cuda") == 1              # the first is past the pool, the second a padding row
+    written = kc.view(torch.uint8).view(32, -1).any(-1).nonzero().flatten().tolist()
+    assert written == [7]

@@ -72,6 +72,7 @@ SIGNATURES = {
         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_int,
         c_void_p, POINTER(DecodePlanInfo), c_int, c_int, c_int, c_int, c_int, c_float,
         c_void_p, c_size_t, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "b200_call_fp8": (c_int, [c_int, c_char_p]),
     "b200_prefill_plan_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "b200_prefill_plan": (c_int, [
         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,

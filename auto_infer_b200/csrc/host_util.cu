@@ -5,6 +5,9 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <tuple>
+#include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "fp8.cuh"
@@ -188,9 +191,50 @@ int get_fp8_cache_tensor_map(const void* cache, int num_blocks, int block_size, 
   return B200_OK;
 }
 
+// One 8-byte word of an argument block as the type the entry point declares.
+template <class T>
+T from_word(int64_t w, bool& fits) {
+  if constexpr (std::is_pointer_v<T>) {
+    return reinterpret_cast<T>(w);
+  } else if constexpr (std::is_floating_point_v<T>) {
+    double d;
+    memcpy(&d, &w, sizeof(d));
+    return static_cast<T>(d);
+  } else {
+    fits = fits && static_cast<int64_t>(static_cast<T>(w)) == w && (std::is_signed_v<T> || w >= 0);
+    return static_cast<T>(w);
+  }
+}
+template <class... Args, size_t... kI>
+int call_block(int (*entry)(Args...), const int64_t* words, std::index_sequence<kI...>) {
+  bool fits = true;
+  std::tuple<Args...> args{from_word<Args>(words[kI], fits)...};
+  if (!fits) {
+    set_last_error("call_fp8: an integer does not fit its argument");
+    return B200_EINVAL;
+  }
+  return std::apply(entry, args);
+}
+template <class... Args>
+int call_block(int (*entry)(Args...), const int64_t* words) {
+  return call_block(entry, words, std::index_sequence_for<Args...>{});
+}
+
 }  // namespace b200
 
 extern "C" {
+
+int b200_call_fp8(int entry, const void* args) {
+  using namespace b200;
+  const int64_t* words = static_cast<const int64_t*>(args);
+  if (words && reinterpret_cast<uintptr_t>(words) % 8 == 0) {
+    if (entry == B200_CALL_RESHAPE_AND_CACHE_FP8) return call_block(b200_reshape_and_cache_fp8, words);
+    if (entry == B200_CALL_PAGED_DECODE_GQA_FP8) return call_block(b200_paged_decode_gqa_fp8, words);
+    if (entry == B200_CALL_PAGED_PREFILL_GQA_FP8) return call_block(b200_paged_prefill_gqa_fp8, words);
+  }
+  set_last_error("call_fp8: unknown entry %d, or an argument block that is null or not 8-byte aligned", entry);
+  return B200_EINVAL;
+}
 
 const char* b200_version(void) { return "b200-attention 0.1 sm_100a"; }
 

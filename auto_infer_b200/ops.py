@@ -4,6 +4,7 @@ tensors.  CPU tensors are rejected: there is no host implementation."""
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -13,6 +14,7 @@ from ._lib import DecodePlanInfo, PrefillPlanInfo
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # without the initialisation check
 
 
 def _stream_ptr(device) -> int:
@@ -135,26 +137,35 @@ def _status_ptr(index: int) -> int:
     return _status_ptrs[index]
 
 
+# The calls over an 8-bit cache as ``b200_call_fp8`` takes them: number, and the arguments in one block (ctypes converts
+# 27 arguments one by one in about the time of the launch)
+_CALLS = {name: (number, struct.Struct("".join("d" if t is ctypes.c_float else "q" for t in _lib.SIGNATURES[name][1])))
+          for number, name in enumerate(("b200_reshape_and_cache_fp8", "b200_paged_decode_gqa_fp8",
+                                         "b200_paged_prefill_gqa_fp8"))}
+
+
 def _call_on(index: int, name: str, *args) -> None:
     """Library call ``name`` with device ``index`` current; the status word and torch's current stream of that
-    device are appended to ``args``."""
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, _status_ptr(index), _stream_ptr(torch.device("cuda", index)) if _raw_stream is None
-                else _raw_stream(index))
+    device are appended to ``args`` (null pointers are 0)."""
+    lib = _lib._lib or _lib.load()
+    number, block = _CALLS[name]
+    status = _status_ptrs.get(index) or _status_ptr(index)
+    if _current_device() == index:
+        rc = lib.b200_call_fp8(number, block.pack(*args, status, _raw_stream(index) if _raw_stream is not None
+                                                  else _stream_ptr(torch.device("cuda", index))))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _status_ptr(index), _stream_ptr(torch.device("cuda", index)))
+            rc = lib.b200_call_fp8(number, block.pack(*args, status, _stream_ptr(torch.device("cuda", index))))
     if rc:
         _lib.check(rc, name)
 
 
 def _check_fp8_cache(key_cache, value_cache, key_scale, value_scale) -> tuple:
     """(num_blocks, block_size, Hkv, D) of an 8-bit cache whose four tensors fit together."""
-    shape = key_cache.shape
+    shape, scales = key_cache.shape, key_scale.shape
     if (key_cache.dtype is _E4M3 and value_cache.dtype is _E4M3 and key_scale.dtype is _F32
             and value_scale.dtype is _F32 and len(shape) == 4 and value_cache.shape == shape
-            and key_scale.shape == (shape[0], shape[2]) and value_scale.shape == key_scale.shape
+            and len(scales) == 2 and scales[0] == shape[0] and scales[1] == shape[2] and value_scale.shape == scales
             and key_cache.is_contiguous() and value_cache.is_contiguous() and key_scale.is_contiguous()
             and value_scale.is_contiguous()):
         return shape
@@ -441,7 +452,8 @@ def _fp8_attention_args(who, kind, q, key_cache, value_cache, key_scale, value_s
     elif block_table.stride(1) != 1:
         block_table = block_table.contiguous()
     if out is None:
-        out = torch.empty_like(q, dtype=_F32 if out_f32 else _BF16, memory_format=torch.contiguous_format)
+        out = (torch.empty(q_shape, dtype=_F32, device=q.device) if out_f32 else torch.empty_like(q) if q.is_contiguous()
+               else torch.empty_like(q, memory_format=torch.contiguous_format))
     elif out.shape != q_shape or out.dtype not in (_BF16, _F32) or not out.is_contiguous():
         raise ValueError(f"{who}: out must be contiguous, of q's shape, torch.bfloat16 or torch.float32")
     if lse_out is not None and (lse_out.shape != (t, n_q) or lse_out.dtype is not _F32
@@ -465,9 +477,9 @@ def paged_decode_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     _call_on(index, "b200_paged_decode_gqa_fp8", q.data_ptr(), q.stride(0), key_cache.data_ptr(),
              value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), num_blocks, block_size,
              block_table.data_ptr(), block_table.stride(0), rows, cols, plan.dev.data_ptr(),
-             None if plan.replayable else ctypes.byref(plan.info), plan.num_ctas, t, n_q, n_kv, d, scale,
+             0 if plan.replayable else ctypes.addressof(plan.info), plan.num_ctas, t, n_q, n_kv, d, scale,
              workspace.data_ptr(), workspace.numel(), out.data_ptr(), out.dtype is _F32,
-             None if lse_out is None else lse_out.data_ptr())
+             0 if lse_out is None else lse_out.data_ptr())
     return out
 
 
@@ -679,8 +691,8 @@ def paged_prefill_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache:
     _call_on(index, "b200_paged_prefill_gqa_fp8", q.data_ptr(), q.stride(0), key_cache.data_ptr(),
              value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), num_blocks, block_size,
              block_table.data_ptr(), block_table.stride(0), rows, cols, plan.dev.data_ptr(),
-             None if plan.replayable else ctypes.byref(plan.info), max_ctas, t, n_q, n_kv, d, scale,
-             out.data_ptr(), out.dtype is _F32, None if lse_out is None else lse_out.data_ptr())
+             0 if plan.replayable else ctypes.addressof(plan.info), max_ctas, t, n_q, n_kv, d, scale,
+             out.data_ptr(), out.dtype is _F32, 0 if lse_out is None else lse_out.data_ptr())
     return out
 
 

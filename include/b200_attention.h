@@ -364,6 +364,16 @@ int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride,
                                void* out, int out_is_f32, float* lse_out,
                                int32_t* status, void* stream);
 
+/* The three calls over an 8-bit cache with their arguments in one block: in the order of the
+ * declarations, 8 bytes each - pointers (NULL: 0) and integers as they are, `scale` as a double.
+ * For bindings that pay for every argument they convert (a ctypes call of 27 costs as much as the
+ * launch).  The block is 8-byte aligned; an integer that does not fit the declaration's type is
+ * refused. */
+#define B200_CALL_RESHAPE_AND_CACHE_FP8 0   /* 16 arguments */
+#define B200_CALL_PAGED_DECODE_GQA_FP8  1   /* 27 */
+#define B200_CALL_PAGED_PREFILL_GQA_FP8 2   /* 25 */
+int b200_call_fp8(int entry, const void* args);
+
 /* ------------------------------------------------------------------------ *
  * Same attention as b200_paged_decode_gqa for callers that may not allocate
  * device memory.  (No counterpart in the reference: its vendor op manages its

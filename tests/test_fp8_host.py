@@ -159,3 +159,33 @@ def test_page_copy_refuses_what_is_not_words(lib):
              status=None, stream=None)
     for change in (dict(page_bytes=6), dict(src=(1 << 20) + 2), dict(dst=(1 << 21) + 1)):
         assert lib.b200_copy_blocks(*(a | change).values()) == -3
+
+
+def _block(entry, args):
+    """The argument block of ``b200_call_fp8``: 8 bytes an argument, `scale` as a double."""
+    import ctypes
+    import struct
+    from auto_infer_b200._lib import SIGNATURES
+    types = SIGNATURES[entry][1]
+    assert len(types) == len(args)
+    words = [ctypes.addressof(a._obj) if hasattr(a, "_obj") else 0 if a is None else a for a in args]
+    return struct.pack("".join("d" if t is ctypes.c_float else "q" for t in types), *words)
+
+
+def test_calls_in_one_block_reach_the_same_checks(lib):
+    """Each refusal of the entry points comes back from the block form, and integers that do not fit are refused."""
+    calls = ((0, "b200_reshape_and_cache_fp8", _write_args, (dict(key_cache=None), dict(head_dim=64), dict(block_size=24),
+                                                             dict(num_tokens=3, key_stride=255), dict(num_tokens=0))),
+             (1, "b200_paged_decode_gqa_fp8", _decode_args, (dict(q=None), dict(num_q_heads=7), dict(head_dim=96),
+                                                             dict(q_stride=1022), dict(workspace_bytes=100),
+                                                             dict(info=None, num_ctas=0))))
+    for number, name, make, changes in calls:
+        for change in changes:
+            assert lib.b200_call_fp8(number, _block(name, make(**change))) == getattr(lib, name)(*make(**change))
+            assert number == 0 or lib.b200_last_error()
+        for field in ("num_blocks", "head_dim"):
+            assert lib.b200_call_fp8(number, _block(name, make(**{field: 2 ** 32 + 128}))) == -1
+            assert b"does not fit" in lib.b200_last_error()
+    assert lib.b200_call_fp8(1, _block(calls[1][1], _decode_args(workspace_bytes=-1))) == -1
+    assert lib.b200_call_fp8(3, b"\0" * 256) == -1 and b"unknown entry 3" in lib.b200_last_error()
+    assert lib.b200_call_fp8(1, None) == -1

@@ -92,7 +92,10 @@ SIGNATURES = {
     "b200_paged_prefill_gqa_fp8": (c_int, [
         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_int,
         c_void_p, POINTER(PrefillPlanInfo), c_int, c_int, c_int, c_int, c_int, c_float,
-        c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+        c_void_p, c_size_t, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "b200_prefill_split_bytes": (c_size_t, [c_int, c_int]),
+    "b200_prefill_split_workspace_bytes": (c_size_t, [c_int]),
+    "b200_prefill_split": (c_int, [c_void_p, c_size_t, c_int, POINTER(PrefillPlanInfo), POINTER(c_int)]),
     "b200_mha_plan_bytes": (c_size_t, [c_int, c_int, c_int]),
     "b200_mha_workspace_bytes": (c_size_t, [c_int, c_int]),
     "b200_mha_plan": (c_int, [

@@ -26,11 +26,19 @@
 // tile of 128 x 128.  A tile takes about 1850 cycles: each group's chain scores -> maximum -> weights -> P is about 3700
 // long, two of them run, and a softmax warp issues an instruction in about three cycles.  Where an item ends, O has
 // to be read before the next item's first P V.  Measured (32 query heads, 8 kv heads): 525 us on an 8192-token prompt (1046
-// TFLOP/s), 106 us on four 512-token chunks over cached prefixes, 41 us on 16 drafts of 5 tokens over 2 to 8
-// thousand tokens.  What else was tried: both groups on row tiles of their own with one K / V stream (620 us: the
+// TFLOP/s), 106 us on four 512-token chunks over cached prefixes, 41 us on 16 drafts of 5 tokens over 512 to 4096
+// tokens.  Where few items meet many SMs the plan cuts them along the keys (b200_prefill_split) and a second kernel joins
+// the pieces: 81 us instead of 985 on 16 rows over 131072 tokens, 85 instead of 262 on 2 x 64 rows over 32768, 53 instead
+// of 69 on 16 drafts over 2048 to 8192.  What else was tried: both groups on row tiles of their own with one K / V stream (620 us: the
 // instruction footprint of two O rescales), the groups' exponential sections kept apart by a barrier (799 us against 742 at
 // the time).  All roles' loops share the SM's instruction cache, so each piece of code is instantiated once and outer
 // loops are not unrolled: from 85 KB of code to 64 KB, with the waits in line, took 742 us to 581.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <exception>
+#include <vector>
+
 #include "fp8.cuh"
 #include "prefill_plan.cuh"
 #include "tc05.cuh"
@@ -43,6 +51,7 @@ constexpr int kP8VStages = 2;                                   // codes; two mo
 constexpr int kP8KLead = 2;                                     // K loads run this many tiles ahead of the V loads
 constexpr int kP8ScaleSlots = 8;
 constexpr int kP8Groups = kPfTile / kFp8MinBlockSize;           // column groups of a tile: 8
+constexpr int kMaxGroups = 1024;                                // cut items of a plan (one per SM at most)
 constexpr int kP8SoftmaxThreads = 256;
 constexpr int kP8ConvertThreads = 128;
 constexpr int kP8Threads = kP8SoftmaxThreads + 128 + kP8ConvertThreads;   // whole warpgroups: 512 = 4 x 128
@@ -89,7 +98,7 @@ struct __align__(1024) Prefill8Smem {
   uint64_t q_empty[2];                     // all S MMAs of the item have run
   uint64_t item_full[2];                   // work-queue hand-off: producer warp -> the other roles
   uint64_t item_empty[2];
-  alignas(16) PrefillItem next_rec[2];     // the mailbox carries the whole item record (read as int4)
+  alignas(16) PrefillPiece next_rec[2];    // the mailbox carries the whole record (read as int4)
   int next_item[2];
   uint32_t tmem_base;
   int abort_flag;
@@ -104,7 +113,9 @@ struct Prefill8Params {
   int64_t bt_stride;
   int table_rows, table_cols;
   int num_tokens;
-  const PrefillItem* items;
+  int32_t* plan;                    // header, items or pieces, groups
+  float* part;                      // partial records of cut items, kPieceRecFloats each
+  int max_partials;                 // records the workspace holds
   int* work_counter;                // two plan words: next item to hand out, CTAs that have left
                                     // (the word before them is the number of items)
   void* out;
@@ -162,7 +173,10 @@ __device__ __forceinline__ void umma_f8_ss_lo(uint32_t tmem_d, uint32_t a_lo, ui
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t}"
       ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(kAccumulate ? 1 : 0));
 }
-template <bool kOnePage>   // pages of 128 tokens or more: one pair of scales per tile
+// kOnePage: pages of 128 tokens or more, one pair of scales per tile.  kCut: a plan that has pieces, or that a recorded
+// launch may find them in (545 us instead of 525 on an 8192-token prompt without any: the roles that walk tiles have no
+// register left for where a piece begins).
+template <bool kOnePage, bool kCut>
 __global__ void __launch_bounds__(kP8Threads, 1)
 paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                          const Prefill8Params p) {
@@ -217,12 +231,15 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
   const uint32_t abort_at = smem_u32(&sm.abort_flag);
   // Items are handed out dynamically, longest first: the producer warp draws the next index from a
   // global counter and passes it to the other roles through a two-slot mailbox.  -1 ends the CTA.
-  auto take_item = [&](uint32_t k, PrefillItem& rec) -> int {
+  auto first_of = [](const PrefillPiece& x) -> int { return kCut ? x.tile_begin : 0; };   // first tile
+  auto take_item = [&](uint32_t k, PrefillPiece& rec) -> int {
     mbar_wait_limited(&sm.item_full[k & 1u], (k >> 1) & 1u, abort_at);
     const int idx = *reinterpret_cast<volatile int*>(&sm.next_item[k & 1u]);
     const int4* src = reinterpret_cast<const int4*>(&sm.next_rec[k & 1u]);
     const int4 lo = src[0], hi = src[1];
-    rec = PrefillItem{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    int2 cut = make_int2(0, -1);
+    if constexpr (kCut) cut = *reinterpret_cast<const int2*>(src + 2);
+    rec = PrefillPiece{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w, cut.x, cut.y, {0, 0}};
     mbar_arrive(&sm.item_empty[k & 1u]);
     return (*abort_flag || idx < 0) ? -1 : idx;
   };
@@ -242,13 +259,16 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         if (lane == 0) {
           // the first item of a CTA is its own index; the rest of the list is handed out dynamically
           idx = (k == 0) ? (int)blockIdx.x : (int)gridDim.x + atomicAdd(p.work_counter, 1);
-          if (idx >= __ldg(p.work_counter - 1) || *abort_flag) idx = -1;
+          const int pieces = kCut ? __ldg(p.plan + kHdrPieces) : 0;    // 0: nothing is cut
+          if (idx >= (pieces ? pieces : __ldg(p.plan + 1)) || *abort_flag) idx = -1;
           mbar_wait_limited(&sm.item_empty[k & 1u], ((k >> 1) & 1u) ^ 1u, abort_at);
           if (idx >= 0) {
-            const int4* src = reinterpret_cast<const int4*>(p.items + idx);
+            const int4* src = reinterpret_cast<const int4*>(
+                p.plan + (pieces ? __ldg(p.plan + kHdrOffPieces) + kPieceInts * idx : kPlanHeaderInts + kPfItemInts * idx));
             int4* dst = reinterpret_cast<int4*>(&sm.next_rec[k & 1u]);
             dst[0] = __ldg(src);
             dst[1] = __ldg(src + 1);
+            if constexpr (kCut) dst[2] = pieces ? __ldg(src + 2) : make_int4(0, -1, 0, 0);
           }
           sm.next_item[k & 1u] = idx;
           mbar_arrive(&sm.item_full[k & 1u]);     // release semantics: index and record are visible to waiters
@@ -259,7 +279,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       const int groups_per_box = p.box_tokens / kFp8MinBlockSize;
       // Each piece of code below is instantiated once: the kernel's loops share one instruction cache.  The walk
       // starts with an item without tiles, whose only step draws item 0.
-      PrefillItem item{};
+      PrefillPiece item{};
       int idx = 0;
 #pragma unroll 1
       for (uint32_t k = 0; idx >= 0; ++k) {          // `item` is item k - 1; item k is drawn on the way
@@ -283,7 +303,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             const uint32_t itx = it + step;
             int bid = -1;
             if (lane < kP8Groups) {
-              int lb = (step * kPfTile + lane * kFp8MinBlockSize) >> p.block_shift;
+              int lb = ((first_of(item) + step) * kPfTile + lane * kFp8MinBlockSize) >> p.block_shift;
               lb = lb > last_block ? last_block : lb;                  // the tail re-reads the last valid page
               if (lb < cols) bid = table[lb];
               if (bid >= p.num_blocks) bid = -1;
@@ -297,7 +317,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             __syncwarp();
             if (lane < nbox)                         // a page outside the pool: TMA fills zeros
               tma_load_4d(sm.k[sk] + box_row * kFp8HeadDim, &k_map, &sm.k_full[sk], 0, item.kv_head,
-                          (step * kPfTile + box_row) & (p.block_size - 1), b < 0 ? p.num_blocks : b);
+                          ((first_of(item) + step) * kPfTile + box_row) & (p.block_size - 1), b < 0 ? p.num_blocks : b);
             // The tile's scales, through a ring of their own: the K stage is handed back before the softmax
             // threads read them.  Slot itx - 8 is free: the K stage this tile takes was freed by S of tile
             // itx - 3, whose score buffer was handed back by the readers of tile itx - 5.
@@ -319,7 +339,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             __syncwarp();
             if (lane < nbox)
               tma_load_4d(sm.v[sv] + box_row * kFp8HeadDim, &v_map, &sm.v_full[sv], 0, item.kv_head,
-                          (tile * kPfTile + box_row) & (p.block_size - 1), b < 0 ? p.num_blocks : b);
+                          ((first_of(item) + tile) * kPfTile + box_row) & (p.block_size - 1), b < 0 ? p.num_blocks : b);
           }
           __syncwarp();
         }
@@ -351,7 +371,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         uint32_t it = 0;
 #pragma unroll 1
         for (uint32_t item_no = 0;; ++item_no) {
-          PrefillItem rec;
+          PrefillPiece rec;
           if (take_item(item_no, rec) < 0) break;
           const int n_tiles = rec.n_tiles;
           const uint32_t qb = item_no & 1u;
@@ -387,7 +407,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         uint32_t it = 0;
 #pragma unroll 1
         for (uint32_t item_no = 0;; ++item_no) {
-          PrefillItem rec;
+          PrefillPiece rec;
           if (take_item(item_no, rec) < 0) break;
           const int n_tiles = rec.n_tiles;
 #pragma unroll 1
@@ -427,12 +447,12 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     uint32_t it = 0;
 #pragma unroll 1
     for (uint32_t item_no = 0;; ++item_no) {
-      PrefillItem item;
+      PrefillPiece item;
       if (take_item(item_no, item) < 0) break;
       const int rg = item.row0 + r;
       const bool valid = rg < item.q_len * G;
       // rows past the item's see whatever there is: nobody reads their O
-      const int lim = valid ? min(item.causal_base + rg / G, item.kv_len - 1) : INT_MAX;
+      const int lim = (valid ? min(item.causal_base + rg / G, item.kv_len - 1) : INT_MAX) - first_of(item) * kPfTile;
       const bool idle = !__any_sync(0xffffffffu, valid);
       mbar_wait_limited(&sm.q_full[item_no & 1u], (item_no >> 1) & 1u, abort_at);
       const float row_factor = sm.row_factor[item_no & 1u][r];
@@ -636,10 +656,11 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       for (int i = 0; i < 2; ++i) raw[i] = q_row ? q_row[2 * step + i] : make_uint4(0u, 0u, 0u, 0u);
     };
     struct Row {                                     // what this thread keeps of an item
-      int n_tiles, kv_len;
+      int n_tiles, kv_len;                           // keys from the item's first tile on
+      int partial;                                   // record of a piece of a cut item, or -1
       int64_t out;                                   // its row e among the rows of `out`, or -1
     };
-    auto begin_q = [&](const PrefillItem& x) -> Row {
+    auto begin_q = [&](const PrefillPiece& x) -> Row {
       const bool fits = x.q_start + x.q_len <= p.num_tokens;
       const int rg = x.row0 + r;
       if (r == 0 && !fits && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
@@ -665,7 +686,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       const int e = max((int)(max(top & 0xffffu, top >> 16) >> 7), 8);
       up = e == 255 ? NAN : __uint_as_float((uint32_t)(261 - e) << 23);   // 2^(7 - (e - 127)); any inf or NaN: the row is NaN
       row_factor = __uint_as_float((uint32_t)(e - 7) << 23) * p.scale_log2;
-      return Row{x.n_tiles, x.kv_len, valid ? tok * p.num_q_heads + head : -1};
+      return Row{x.n_tiles, x.kv_len - first_of(x) * kPfTile, kCut ? x.partial : -1, valid ? tok * p.num_q_heads + head : -1};
     };
     auto put_step = [&](uint32_t k) {
       if (step == 0) {
@@ -742,7 +763,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
     };
     // One instance of each piece of code (see the producer): iteration k works on item k - 1, whose Q was staged in the
     // iteration before; it stages item k behind its own last V tiles and writes item k - 2 behind its first.
-    Row item{}, prev{}, next{};
+    Row item{0, 0, -1, -1}, prev = item, next = item;
     int total = -1;                                  // items of this CTA, once known
 #pragma unroll 1
     for (int k = 0; total < 0 || k < total + 2; ++k) {
@@ -751,7 +772,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
 #pragma unroll 1
       for (int tile = 0; tile == 0 || tile < n || step < kSteps; ++tile) {
         if (total < 0 && tile == take_at) {
-          PrefillItem rec;
+          PrefillPiece rec;
           if (take_item(k, rec) >= 0)
             next = begin_q(rec);
           else
@@ -764,7 +785,12 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         if (tile > 0 || k < 2) continue;
         const uint32_t item_no = k - 2;
         // ---- epilogue: row e of O out of tensor memory as soon as the item's last P V has run
-        const bool valid = prev.out >= 0;
+        // a piece of a cut item leaves normalised fp32 rows and their log2 sums in its record
+        const bool cut = kCut && prev.partial >= 0, to_f32 = cut || p.out_is_f32;
+        const bool fits = !kCut || prev.partial < p.max_partials, valid = prev.out >= 0 && fits;
+        if (!fits && r == 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
+        uint8_t* const row_at = cut ? reinterpret_cast<uint8_t*>(p.part + (int64_t)prev.partial * kPieceRecFloats + r * kPfHeadDim)
+                                    : static_cast<uint8_t*>(p.out) + prev.out * (kPfHeadDim * (to_f32 ? 4 : 2));
         mbar_wait_limited(&sm.l_full, item_no & 1u, abort_at);
         const float m0 = sm.row_m[0][r], m1 = sm.row_m[1][r], mo = sm.row_mfin[r];
         const float mm = fmaxf(m0, m1);
@@ -802,14 +828,12 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             for (int i = 0; i < 32; ++i) o[i] = 0u;
           }
           if (valid) {
-            const int64_t off = prev.out * kPfHeadDim + q4 * 32;
-            if (p.out_is_f32) {
-              float* dst = reinterpret_cast<float*>(p.out) + off;
+            if (to_f32) {
+              uint4* dst = reinterpret_cast<uint4*>(row_at + q4 * 128);
 #pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<uint4*>(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             } else {
-              __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + off;
+              uint4* dst = reinterpret_cast<uint4*>(row_at + q4 * 64);
 #pragma unroll
               for (int i = 0; i < 32; i += 8) {
                 uint4 v;
@@ -817,13 +841,17 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                 v.y = pack_bf16(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
                 v.z = pack_bf16(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
                 v.w = pack_bf16(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
-                *reinterpret_cast<uint4*>(dst + i) = v;
+                dst[i >> 3] = v;
               }
             }
           }
         }
-        if (valid && p.lse_out)
-          p.lse_out[prev.out] = empty ? -INFINITY : mm * 0.6931471805599453f + __logf(lsum);
+        if (valid) {
+          if (kCut && prev.partial >= 0)
+            p.part[(int64_t)prev.partial * kPieceRecFloats + kPfRows * kPfHeadDim + r] = empty ? -INFINITY : mm + fast_log2(lsum);
+          else if (p.lse_out)
+            p.lse_out[prev.out] = empty ? -INFINITY : mm * 0.6931471805599453f + __logf(lsum);
+        }
       }
       prev = item;
       item = next;
@@ -849,7 +877,140 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
   }
 }
 
+// Joins the pieces of cut items, a warp a row: the rows of a piece are normalised, the weights of the pieces are
+// their sums 2^(log2 sum).  The order of the tiles is the order of the sum.  Bound by latency (at most 20 MB of records).
+// A kernel of its own: inside the other one, by the last CTA to arrive, its registers cost every item 4 % and more.
+__global__ void __launch_bounds__(256)
+prefill_join_kernel(const Prefill8Params p) {
+  grid_dep_wait();
+  const int first_group = p.plan[kHdrOffGroups];
+  // groups lie behind the pieces, to the end of what the header counts
+  if (p.plan[kHdrPieces] == 0 || (int)blockIdx.x >= p.plan[kHdrGroups]) return;
+  const PieceGroup g = reinterpret_cast<const PieceGroup*>(p.plan + first_group)[blockIdx.x];
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rg = g.row0 + r;
+  if (rg >= g.q_len * p.group || g.q_start + g.q_len > p.num_tokens || g.part_begin + g.n_parts > p.max_partials) return;
+  const float* const rec = p.part + (int64_t)g.part_begin * kPieceRecFloats;
+  const float* const sums = rec + kPfRows * kPfHeadDim + r;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < g.n_parts; ++i) top = fmaxf(top, sums[(int64_t)i * kPieceRecFloats]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float total = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < g.n_parts; ++i) {
+    const float w = fast_exp2(sums[(int64_t)i * kPieceRecFloats] - ref);
+    const float4 y = *reinterpret_cast<const float4*>(rec + (int64_t)i * kPieceRecFloats + r * kPfHeadDim + 4 * lane);
+    total += w;
+    acc.x += w * y.x;
+    acc.y += w * y.y;
+    acc.z += w * y.z;
+    acc.w += w * y.w;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int64_t row = (int64_t)(g.q_start + rg / p.group) * p.num_q_heads + g.kv_head * p.group + rg % p.group;
+  if (p.out_is_f32) {
+    reinterpret_cast<float4*>(p.out)[row * 32 + lane] = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  } else {
+    reinterpret_cast<uint2*>(p.out)[row * 32 + lane] =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+  if (p.lse_out && lane == 0) p.lse_out[row] = total == 0.f ? -INFINITY : (top + fast_log2(total)) * 0.6931471805599453f;
+}
+
 }  // namespace b200
+
+// Bytes that the pieces and groups of a plan of at most num_items items take at its end.
+extern "C" size_t b200_prefill_split_bytes(int num_items, int num_ctas) {
+  using namespace b200;
+  if (num_items < 0 || num_ctas <= 0) return 0;
+  return sizeof(PrefillPiece) * ((size_t)num_items + num_ctas) + sizeof(PieceGroup) * (size_t)num_ctas;
+}
+extern "C" size_t b200_prefill_split_workspace_bytes(int num_partials) {
+  return num_partials < 0 ? 0 : sizeof(float) * b200::kPieceRecFloats * (size_t)num_partials;
+}
+
+// Where few items meet many SMs the longest sets the time.  The tiles are then dealt to num_ctas equal shares in the
+// order of the list, items are cut where a share ends, and the pieces are sorted by length: handed out longest first, the
+// big ones fill most of a share and the small ones what is left.
+extern "C" int b200_prefill_split(int32_t* plan, size_t plan_bytes, int num_ctas, b200_prefill_plan_info* info,
+                                  int* num_partials) try {
+  using namespace b200;
+  if (!plan || !info || !num_partials || num_ctas <= 0 || num_ctas > kMaxGroups || plan[0] != kPfMagic || info->num_items != plan[1]) {
+    set_last_error("prefill_split: null pointer, no CTAs, or not a plan of b200_prefill_plan");
+    return B200_EINVAL;
+  }
+  const int n = info->num_items;
+  const PrefillItem* items = reinterpret_cast<const PrefillItem*>(plan + kPlanHeaderInts);
+  const int base = kPlanHeaderInts + kPfItemInts * n;
+  if (plan_bytes < base * sizeof(int32_t) + b200_prefill_split_bytes(n, num_ctas)) {
+    set_last_error("prefill_split: plan buffer of %zu bytes is smaller than b200_prefill_split_bytes() asks for", plan_bytes);
+    return B200_EPLAN;
+  }
+  for (int i = kHdrPieces; i <= kHdrGroups; ++i) plan[i] = 0;
+  info->plan_ints = base;
+  *num_partials = 0;
+  // What an item or piece costs besides its tiles, and a merge, in tiles (the list is sorted: items[0] is the longest)
+  constexpr float kItemCost = 6.f, kMergeCost = 4.f;
+  constexpr int kLeast = 4;                                  // tiles of a piece
+  int64_t total = 0;
+  for (int i = 0; i < n; ++i) total += items[i].n_tiles;
+  if (n == 0 || total == 0 || n > 4 * num_ctas) return B200_OK;
+  const float longest = (float)items[0].n_tiles, share = (float)total / num_ctas, rounds = (float)n / num_ctas;
+  const int per = std::max((int)std::ceil(share), 2 * kLeast);
+  const float whole = rounds <= 1.f ? longest + kItemCost
+                                    : std::min(std::ceil(rounds) * (longest + kItemCost),
+                                               share + longest / 2 + kItemCost * (rounds + 1));
+  const float cut = per + kItemCost * (rounds + 2) + kMergeCost;
+  if (cut > 0.93f * whole) return B200_OK;
+
+  std::vector<PrefillPiece> pieces;
+  std::vector<PieceGroup> groups;
+  pieces.reserve(n + num_ctas);
+  int room = per, spare = num_ctas;                          // tiles left of the share; cuts the buffer has room for
+  for (int i = 0; i < n; ++i) {
+    const PrefillItem& x = items[i];
+    const size_t first = pieces.size();
+    int begin = 0;
+    do {
+      const int left = x.n_tiles - begin;
+      int take = std::min(left, room);
+      if (left - take < kLeast || spare == 0) take = left;   // no sliver behind a cut
+      if (take < left) --spare;
+      pieces.push_back(PrefillPiece{x.seq, x.kv_head, x.row0, take, x.kv_len, x.q_start, x.q_len, x.causal_base, begin,
+                                    -1, 0, 0});
+      begin += take;
+      room -= take;
+      if (room < kLeast) room += per;
+    } while (begin < x.n_tiles);
+    const int parts = (int)(pieces.size() - first);
+    if (parts > 1) {
+      for (int k = 0; k < parts; ++k) pieces[first + k].partial = *num_partials + k;
+      groups.push_back(PieceGroup{*num_partials, parts, x.kv_head, x.row0, x.q_start, x.q_len, 0, 0});
+      *num_partials += parts;
+    }
+  }
+  if (groups.empty()) return B200_OK;
+  // longest first, by counting: the list is made on the way of a step
+  const int most = (int)longest + kLeast;
+  std::vector<int> at(most + 2, 0);
+  for (const PrefillPiece& x : pieces) ++at[most - std::min(x.n_tiles, most) + 1];
+  for (int k = 0; k <= most; ++k) at[k + 1] += at[k];
+  PrefillPiece* sorted = reinterpret_cast<PrefillPiece*>(plan + base);
+  for (const PrefillPiece& x : pieces) sorted[at[most - std::min(x.n_tiles, most)]++] = x;
+  const int off_groups = base + kPieceInts * (int)pieces.size();
+  memcpy(plan + off_groups, groups.data(), groups.size() * sizeof(PieceGroup));
+  plan[kHdrPieces] = (int)pieces.size();
+  plan[kHdrOffPieces] = base;
+  plan[kHdrOffGroups] = off_groups;
+  plan[kHdrGroups] = (int)groups.size();
+  info->plan_ints = off_groups + kPieceGroupInts * (int)groups.size();
+  return B200_OK;
+} catch (const std::exception& e) {
+  b200::set_last_error("prefill_split: %s", e.what());
+  return B200_ETOOLARGE;
+}
 
 extern "C" int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride, const void* key_cache,
                                           const void* value_cache, const float* key_scale,
@@ -857,8 +1018,8 @@ extern "C" int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride, const
                                           const int32_t* block_table, int64_t bt_stride, int table_rows,
                                           int table_cols, int32_t* plan_dev, const b200_prefill_plan_info* info,
                                           int max_ctas, int num_tokens, int num_q_heads, int num_kv_heads,
-                                          int head_dim, float scale, void* out, int out_is_f32, float* lse_out,
-                                          int32_t* status, void* stream) {
+                                          int head_dim, float scale, void* workspace, size_t workspace_bytes, void* out,
+                                          int out_is_f32, float* lse_out, int32_t* status, void* stream) {
   using namespace b200;
   const char* who = "paged_prefill_gqa_fp8";
   int rc = check_fp8_cache(who, key_cache, value_cache, key_scale, value_scale, num_blocks, block_size, num_kv_heads,
@@ -871,8 +1032,9 @@ extern "C" int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride, const
     return B200_EINVAL;
   }
   if (reinterpret_cast<uintptr_t>(q) % 16 || q_stride % 8 || q_stride < (int64_t)num_q_heads * head_dim ||
-      reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(plan_dev) % 16) {
-    set_last_error("%s: q, out and the plan must be 16-byte aligned, the q token stride a multiple of 8 elements and >= Hq*D", who);
+      reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(plan_dev) % 16 ||
+      reinterpret_cast<uintptr_t>(workspace) % 16) {
+    set_last_error("%s: q, out, plan and workspace must be 16-byte aligned, the q token stride a multiple of 8 elements and >= Hq*D", who);
     return B200_EALIGN;
   }
   const int box_tokens = block_size < kPfTile ? block_size : kPfTile;
@@ -892,7 +1054,10 @@ extern "C" int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride, const
   p.table_rows = table_rows;
   p.table_cols = table_cols;
   p.num_tokens = num_tokens;
-  p.items = reinterpret_cast<const PrefillItem*>(plan_dev + kPlanHeaderInts);
+  p.plan = plan_dev;
+  p.part = static_cast<float*>(workspace);
+  const size_t records = workspace ? workspace_bytes / (kPieceRecFloats * sizeof(float)) : 0;
+  p.max_partials = records > INT32_MAX ? INT32_MAX : (int)records;
   p.work_counter = plan_dev + 2;
   p.out = out;
   p.lse_out = lse_out;
@@ -909,22 +1074,30 @@ extern "C" int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride, const
   p.scale_log2 = scale * 1.4426950408889634f;
 
   const bool one_page = block_size >= kPfTile;
-  auto kernel = one_page ? paged_prefill_fp8_kernel<true> : paged_prefill_fp8_kernel<false>;
+  const bool cut = records > 0;
+  auto kernel = one_page ? (cut ? paged_prefill_fp8_kernel<true, true> : paged_prefill_fp8_kernel<true, false>)
+                         : (cut ? paged_prefill_fp8_kernel<false, true> : paged_prefill_fp8_kernel<false, false>);
   const size_t smem = sizeof(Prefill8Smem);
-  static bool attr_set[2][64] = {{false}, {false}};
+  static bool attr_set[4][64] = {{false}};
+  const int variant = 2 * one_page + cut;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 64 || !attr_set[one_page][dev]) {
+  if (dev >= 64 || !attr_set[variant][dev]) {
     rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                     "paged_prefill_gqa_fp8 smem attribute");
     if (rc) return rc;
-    if (dev < 64) attr_set[one_page][dev] = true;
+    if (dev < 64) attr_set[variant][dev] = true;
   }
   int grid = b200_sm_count();
   if (grid <= 0) grid = 148;
-  if (info && grid > info->num_items) grid = info->num_items;
+  if (info && !records && grid > info->num_items) grid = info->num_items;     // a cut plan has more pieces than items
   if (max_ctas > 0 && grid > max_ctas) grid = max_ctas;     // the rest of the SMs are left to another kernel
-  return check_cuda(launch_pdl(kernel, dim3(grid), dim3(kP8Threads), smem, static_cast<cudaStream_t>(stream), k_map,
-                               v_map, p),
-                    "paged_prefill_gqa_fp8 launch");
+  rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(kP8Threads), smem, static_cast<cudaStream_t>(stream), k_map, v_map,
+                             p),
+                  "paged_prefill_gqa_fp8 launch");
+  const int groups = p.max_partials / 2 < kMaxGroups ? p.max_partials / 2 : kMaxGroups;   // a cut item has two records or more
+  if (rc || groups == 0) return rc;
+  return check_cuda(launch_pdl(prefill_join_kernel, dim3(groups, kPfRows / 8), dim3(256), 0,
+                               static_cast<cudaStream_t>(stream), p),
+                    "paged_prefill_gqa_fp8 join launch");
 }

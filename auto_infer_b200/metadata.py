@@ -94,13 +94,15 @@ class StepMetadata:
     def __init__(self, cu_seqlens_q: Sequence[int], seqlens_kv: Sequence[int], num_q_heads: int,
                  num_kv_heads: int, head_dim: int, device, causal_base: Optional[Sequence[int]] = None,
                  num_ctas: Optional[int] = None, capacity_seqs: Optional[int] = None,
-                 prefill_ctas: int = 0):
+                 prefill_ctas: int = 0, split_prefill: bool = False):
         """``prefill_ctas`` > 0: the step's two kernels are meant to run side by side, the
         wide-query kernel on that many SMs and the decode kernel (planned here for the rest) on
-        the others; see ``mixed_split``."""
+        the others; see ``mixed_split``.  ``split_prefill``: long items of the prefill plan may be cut for the
+        kernel over an 8-bit cache."""
         self.num_q_heads, self.num_kv_heads, self.head_dim = num_q_heads, num_kv_heads, head_dim
         self.device = device
         self.prefill_ctas = int(prefill_ctas)
+        self._split_ctas = (self.prefill_ctas or None) if split_prefill else 0
         if self.prefill_ctas:
             num_ctas = (int(num_ctas) if num_ctas else ops.sm_count(torch.device(device))) - self.prefill_ctas
             if num_ctas < 1:
@@ -141,7 +143,8 @@ class StepMetadata:
                                            self.num_kv_heads, self.device, min_rows=16,
                                            causal_base=causal_base,
                                            capacity_tokens=self.num_tokens if replay else None,
-                                           capacity_seqs=self.decode.capacity_seqs if replay else None)
+                                           capacity_seqs=self.decode.capacity_seqs if replay else None,
+                                           split_ctas=self._split_ctas)
 
     @property
     def capacity_seqs(self) -> int:
@@ -203,7 +206,7 @@ def step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int, devic
                 capacity = max(16, 1 << (max(len(ctx.cu_seqlens_q), 1) - 1).bit_length())
             meta = StepMetadata(ctx.cu_seqlens_q, ctx.seqlens_kv, num_q_heads, num_kv_heads, head_dim,
                                 device, causal_base=causal_base, capacity_seqs=capacity,
-                                prefill_ctas=prefill_ctas)
+                                prefill_ctas=prefill_ctas, split_prefill=kv_elem_bytes == 1)
             if pool is not None:
                 pool[pool_key] = meta
         cache[key] = meta

@@ -553,12 +553,16 @@ class PrefillPlan:
     With ``capacity_tokens`` (and ``capacity_seqs``) the plan is *replayable*: its device
     buffer is sized for any step of at most that many query tokens and sequences and keeps
     its address, ``refill()`` overwrites it in place and the attention launch does not depend
-    on the step, so a CUDA graph that recorded it serves later steps."""
+    on the step, so a CUDA graph that recorded it serves later steps.
+
+    Where the items are few, long ones are cut along the keys for the kernel over an 8-bit cache
+    (``paged_prefill_gqa_fp8``); ``split_ctas`` is the number of SMs its launch will have (default
+    all of the device, 0: never cut).  The plan owns the workspace of the partial results."""
 
     def __init__(self, cu_seqlens_q: Sequence[int], seqlens_kv: Sequence[int], num_q_heads: int,
                  num_kv_heads: int, device, min_rows: int = 16,
                  causal_base: Optional[Sequence[int]] = None, capacity_tokens: Optional[int] = None,
-                 capacity_seqs: Optional[int] = None):
+                 capacity_seqs: Optional[int] = None, split_ctas: Optional[int] = None):
         lib = _lib.load()
         self.device = torch.device(device)
         if self.device.type != "cuda":
@@ -571,6 +575,9 @@ class PrefillPlan:
         self.capacity_seqs = max(int(capacity_seqs or 0), num_seqs) if self.replayable else num_seqs
         self._nbytes = max(lib.b200_prefill_plan_bytes(self.capacity_seqs, self.capacity_tokens, num_q_heads,
                                                        num_kv_heads), 64)
+        self._split_ctas = sm_count(self.device) if split_ctas is None else int(split_ctas)
+        if self._split_ctas:
+            self._nbytes += lib.b200_prefill_split_bytes(self._nbytes // 32, self._split_ctas)   # an item has 32 bytes
         self._hosts = [torch.empty(self._nbytes // 4, dtype=torch.int32, pin_memory=True)
                        for _ in range(2 if self.replayable else 1)]
         self._copied = [None] * len(self._hosts)
@@ -582,6 +589,9 @@ class PrefillPlan:
         self.dev = torch.zeros(self._nbytes // 4 if self.replayable else used, dtype=torch.int32,
                                device=self.device)
         self._upload(used)
+        records = 2 * self._split_ctas if self.replayable else self._num_partials
+        self.workspace = torch.empty(lib.b200_prefill_split_workspace_bytes(records), dtype=torch.uint8,
+                                     device=self.device) if records else None
 
     def _build(self, cu_seqlens_q, seqlens_kv, causal_base) -> None:
         lib = _lib.load()
@@ -599,6 +609,13 @@ class PrefillPlan:
         rc = lib.b200_prefill_plan(cu, kv, base, num_seqs, self.num_q_heads, self.num_kv_heads, self.min_rows,
                                    self.host.data_ptr(), self.host.numel() * 4, ctypes.byref(self.info))
         _lib.check(rc, "b200_prefill_plan")
+        self._num_partials = 0
+        if self._split_ctas:
+            partials = ctypes.c_int(0)
+            rc = lib.b200_prefill_split(self.host.data_ptr(), self.host.numel() * 4, self._split_ctas,
+                                        ctypes.byref(self.info), ctypes.byref(partials))
+            _lib.check(rc, "b200_prefill_split")
+            self._num_partials = partials.value
 
     def _upload(self, used: int) -> None:
         self.dev[:used].copy_(self.host[:used], non_blocking=True)
@@ -688,10 +705,13 @@ def paged_prefill_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache:
         lse_out)
     t, n_q, _ = q.shape
     rows, cols = block_table.shape
+    # a recorded launch must be ready for any step; another knows whether this one's items are cut
+    workspace = plan.workspace if plan._num_partials or plan.replayable and torch.cuda.is_current_stream_capturing() else None
     _call_on(index, "b200_paged_prefill_gqa_fp8", q.data_ptr(), q.stride(0), key_cache.data_ptr(),
              value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), num_blocks, block_size,
              block_table.data_ptr(), block_table.stride(0), rows, cols, plan.dev.data_ptr(),
              0 if plan.replayable else ctypes.addressof(plan.info), max_ctas, t, n_q, n_kv, d, scale,
+             0 if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(),
              out.data_ptr(), out.dtype is _F32, 0 if lse_out is None else lse_out.data_ptr())
     return out
 

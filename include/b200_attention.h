@@ -345,9 +345,24 @@ int b200_paged_prefill_gqa_replayable(const void* q, int64_t q_stride,
                                       void* out, int out_is_f32, float* lse_out,
                                       int32_t* status, void* stream);
 
+/* Cuts long items of a host plan along the keys, for the 8-bit kernel (the 16-bit kernel goes
+ * on reading the uncut items): a step of few items, a draft of some tokens over a long context
+ * for one, would otherwise keep most SMs waiting for the longest.  The plan is left as it is where
+ * that is not expected to pay; the choice depends on the plan and num_ctas (the SMs the launch
+ * will have) only.  Needs b200_prefill_split_bytes(num_items, num_ctas) beyond
+ * b200_prefill_plan_bytes(); info->plan_ints becomes what is used.  The launch's workspace holds
+ * *num_partials records, b200_prefill_split_workspace_bytes(*num_partials); a plan never has
+ * more than 2 * num_ctas. */
+size_t b200_prefill_split_bytes(int num_items, int num_ctas);
+size_t b200_prefill_split_workspace_bytes(int num_partials);
+int b200_prefill_split(int32_t* plan_host, size_t plan_bytes, int num_ctas,
+                       b200_prefill_plan_info* info, int* num_partials);
+
 /* The wide-query attention over an 8-bit cache (layout and scales as
- * b200_reshape_and_cache_fp8).  Plans, masks, q, out and lse_out as
- * b200_paged_prefill_gqa; max_ctas > 0 keeps it to that many SMs as _on does; with
+ * b200_reshape_and_cache_fp8).  Plans (cut or not), masks, q, out and lse_out as
+ * b200_paged_prefill_gqa; workspace 16-byte aligned, NULL where the
+ * plan is known not to be cut (the launch then costs less); a plan that needs more than it holds
+ * sets B200_STATUS_BAD_LAUNCH; max_ctas > 0 keeps it to that many SMs as _on does; with
  * info == NULL the launch is the replayable one.  block_size, table_rows,
  * table_cols, num_tokens and the scales as b200_paged_decode_gqa_fp8.  Cache rows
  * past a sequence's kv_len may hold any codes; a NaN code of V in a row that one
@@ -361,6 +376,7 @@ int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride,
                                int table_rows, int table_cols,
                                int32_t* plan_dev, const b200_prefill_plan_info* info, int max_ctas,
                                int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, float scale,
+                               void* workspace, size_t workspace_bytes,
                                void* out, int out_is_f32, float* lse_out,
                                int32_t* status, void* stream);
 
@@ -371,7 +387,7 @@ int b200_paged_prefill_gqa_fp8(const void* q, int64_t q_stride,
  * refused. */
 #define B200_CALL_RESHAPE_AND_CACHE_FP8 0   /* 16 arguments */
 #define B200_CALL_PAGED_DECODE_GQA_FP8  1   /* 27 */
-#define B200_CALL_PAGED_PREFILL_GQA_FP8 2   /* 25 */
+#define B200_CALL_PAGED_PREFILL_GQA_FP8 2   /* 27 */
 int b200_call_fp8(int entry, const void* args);
 
 /* ------------------------------------------------------------------------ *

@@ -91,7 +91,7 @@ def test_decode_refusals(lib, change, code):
     (dict(q=None), -1), (dict(block_table=None), -1), (dict(plan=None), -1), (dict(out=None), -1), (dict(value_scale=None), -1),
     (dict(num_q_heads=7), -1), (dict(num_tokens=-1), -1), (dict(max_ctas=-1), -1), (dict(table_cols=0), -1),
     (dict(head_dim=256), -2), (dict(block_size=8), -2), (dict(q=(1 << 20) + 8), -3), (dict(q_stride=1028), -3),
-    (dict(out=(1 << 29) + 8), -3), (dict(plan=(1 << 27) + 4), -3),
+    (dict(out=(1 << 29) + 8), -3), (dict(plan=(1 << 27) + 4), -3), (dict(workspace=8), -3),
 ])
 def test_prefill_refusals(lib, change, code):
     from auto_infer_b200._lib import PrefillPlanInfo
@@ -100,7 +100,7 @@ def test_prefill_refusals(lib, change, code):
     a = dict(q=1 << 20, q_stride=1024, key_cache=1 << 22, value_cache=1 << 23, key_scale=1 << 24, value_scale=1 << 25,
              num_blocks=4, block_size=16, block_table=1 << 26, bt_stride=4, table_rows=1, table_cols=4, plan=1 << 27,
              info=ctypes.byref(info), max_ctas=0, num_tokens=1, num_q_heads=8, num_kv_heads=2, head_dim=128, scale=0.1,
-             out=1 << 29, out_is_f32=0, lse_out=None, status=None, stream=None)
+             workspace=None, workspace_bytes=0, out=1 << 29, out_is_f32=0, lse_out=None, status=None, stream=None)
     a.update(change)
     assert lib.b200_paged_prefill_gqa_fp8(*a.values()) == code
     assert b"paged_prefill_gqa_fp8" in lib.b200_last_error()
@@ -189,3 +189,58 @@ def test_calls_in_one_block_reach_the_same_checks(lib):
     assert lib.b200_call_fp8(1, _block(calls[1][1], _decode_args(workspace_bytes=-1))) == -1
     assert lib.b200_call_fp8(3, b"\0" * 256) == -1 and b"unknown entry 3" in lib.b200_last_error()
     assert lib.b200_call_fp8(1, None) == -1
+
+
+@pytest.mark.parametrize("cu, kv, n_kv, ctas", [
+    ([5], [9000], 1, 148), ([5, 10, 15], [9000, 200, 40], 2, 148), ([40] * 3, [5000, 1, 0], 8, 148), ([2000], [2000], 1, 148),
+    ([1, 2, 3], [100000, 70000, 3], 3, 20), ([16], [130], 1, 148), ([0], [50], 2, 4), ([3], [0], 2, 4), ([700], [40000], 1, 1)])
+def test_a_cut_plan_covers_every_tile_once(lib, cu, kv, n_kv, ctas):
+    """The pieces are the items' tiles, each once; records are dealt in the order of the tiles; nothing is a sliver."""
+    import ctypes
+    from auto_infer_b200._lib import PrefillPlanInfo
+    n_q, n = 4 * n_kv, len(cu)
+    ints = lambda x: (ctypes.c_int32 * len(x))(*x)
+    size = lib.b200_prefill_plan_bytes(n, cu[-1], n_q, n_kv)
+    size += lib.b200_prefill_split_bytes(size // 32, ctas)
+    plan = torch.full((size // 4 + 8,), -7, dtype=torch.int32)
+    info, partials = PrefillPlanInfo(), ctypes.c_int(-1)
+    assert lib.b200_prefill_plan(ints(cu), ints(kv), None, n, n_q, n_kv, 0, plan.data_ptr(), size, ctypes.byref(info)) == 0
+    before = plan[:info.plan_ints].clone()
+    assert lib.b200_prefill_split(plan.data_ptr(), size, ctas, ctypes.byref(info), ctypes.byref(partials)) == 0
+    items = before[16:16 + 8 * info.num_items].view(-1, 8)
+    assert torch.equal(plan[16:16 + 8 * info.num_items].view(-1, 8), items) and (plan[info.plan_ints:] == -7).sum() >= 8
+    pieces, at, groups_at, groups = plan[4:8].tolist()
+    assert partials.value <= 2 * ctas and info.plan_ints * 4 <= size
+    if pieces == 0:
+        assert partials.value == 0 and torch.equal(plan[:info.plan_ints], before)
+        return
+    rows = plan[at:at + 12 * pieces].view(-1, 12)
+    assert (rows[:-1, 3] >= rows[1:, 3]).all() and pieces <= info.num_items + ctas
+    parts = {}
+    for x in rows.tolist():
+        parts.setdefault((x[0], x[1], x[2]), []).append((x[8], x[3], x[9]))
+    seen = []
+    for item in items.tolist():
+        runs = sorted(parts.pop((item[0], item[1], item[2])))
+        assert runs[0][0] == 0 and sum(r[1] for r in runs) == item[3]
+        for a, b in zip(runs, runs[1:]):
+            assert a[0] + a[1] == b[0] and b[2] == a[2] + 1 and min(a[1], b[1]) >= 4
+        assert (runs[0][2] == -1) == (len(runs) == 1)
+        if len(runs) > 1:
+            seen.append([runs[0][2], len(runs), item[1], item[2], item[5], item[6]])
+    assert not parts and groups == len(seen)
+    assert plan[groups_at:groups_at + 8 * groups].view(-1, 8)[:, :6].tolist() == seen
+    assert sum(s[1] for s in seen) == partials.value
+
+
+def test_split_refusals(lib):
+    import ctypes
+    from auto_infer_b200._lib import PrefillPlanInfo
+    plan, info, partials = torch.zeros(64, dtype=torch.int32), PrefillPlanInfo(), ctypes.c_int(0)
+    args = [plan.data_ptr(), 256, 148, ctypes.byref(info), ctypes.byref(partials)]
+    assert lib.b200_prefill_split(*args) == -1                               # not a plan
+    assert lib.b200_prefill_plan(None, None, None, 0, 8, 2, 0, plan.data_ptr(), 256, ctypes.byref(info)) == 0
+    assert lib.b200_prefill_split(*args) == -6                               # no room
+    assert lib.b200_prefill_split(None, *args[1:]) == -1 and lib.b200_prefill_split(*args[:2], 0, *args[3:]) == -1
+    assert lib.b200_prefill_split(*args[:2], 5000, *args[3:]) == -1
+    assert lib.b200_prefill_split_bytes(-1, 4) == 0 and lib.b200_prefill_split_workspace_bytes(-1) == 0

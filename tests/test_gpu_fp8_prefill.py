@@ -327,3 +327,68 @@ def test_warps_without_rows(rows):
         _check(first, lse, *c)
         again, lse2 = _run(*c, max_ctas=1)
         assert torch.equal(first, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("lens, q_lens, n_q, n_kv", [
+    ([9000], [5], 8, 1), ([5000, 300, 2], [7, 40, 2], 8, 2), ([4097, 3000, 0], [130, 9, 3], 4, 1), ([20000], [1], 8, 8),
+    ([1500] * 5, [33] * 5, 7, 1), ([130, 6000], [130, 6000 - 5800], 2, 1)])
+@pytest.mark.parametrize("bs", [32, 128])
+def test_items_cut_along_the_keys(lens, q_lens, n_q, n_kv, bs):
+    """Few items over many keys: pieces and their join, with rows that see nothing of the last pieces, into bf16 and
+    fp32, the same bits on any number of CTAs, and what an uncut plan gives within the two's tolerances."""
+    from auto_infer_b200 import ops
+    c = _case(len(lens) + bs, lens, q_lens, n_q, n_kv, bs)
+    plan = ops.PrefillPlan(c[6], c[7], n_q, n_kv, "cuda", min_rows=0)
+    if max(lens) > 2000:                                 # twelve tiles are not worth a cut
+        assert plan.workspace is not None and plan.host[4] > plan.info.num_items and plan.host[7] >= 1
+    first, lse = _run(*c)
+    _check(first, lse, *c)
+    for kw in (dict(max_ctas=3), dict(capacity=c[6][-1] + 4)):
+        again, lse2 = _run(*c, **kw)
+        assert torch.equal(first, again) and torch.equal(lse, lse2)
+    _check(*_run(*c, out_f32=True), *c)
+    whole = ops.PrefillPlan(c[6], c[7], n_q, n_kv, "cuda", min_rows=0, split_ctas=0)
+    assert whole.workspace is None and not whole.host[4:8].any()
+    dev = [x.cuda() for x in c[:6]]
+    lse3 = torch.empty_like(lse, device="cuda")
+    uncut = ops.paged_prefill_gqa_fp8(*dev, whole, c[8], lse_out=lse3)
+    _check(uncut.cpu(), lse3.cpu(), *c)
+    kc = (dev[1].float() * dev[3][:, None, :, None]).to(torch.bfloat16)
+    vc = (dev[2].float() * dev[4][:, None, :, None]).to(torch.bfloat16)
+    wide = [ops.paged_prefill_gqa(dev[0], kc, vc, dev[5], x, c[8]) for x in (plan, whole)]
+    assert torch.equal(wide[0], wide[1])                 # the 16-bit kernel does not see the cuts
+
+
+def test_cut_plans_refilled_and_replayed():
+    """One captured launch for steps that are cut, cut otherwise, not cut, and empty."""
+    from auto_infer_b200 import ops
+    steps = [([9000, 50], [4, 12]), ([700, 6000], [8, 8]), ([60, 60], [8, 8]), ([0, 12000], [1, 15]), ([300, 1], [0, 0])]
+    bs, n_q, n_kv, tokens = 64, 8, 1, 16
+    cases = [_case(k, lens, q_lens, n_q, n_kv, bs) for k, (lens, q_lens) in enumerate(steps)]
+    blocks, width = max(c[1].shape[0] for c in cases), max(c[5].shape[1] for c in cases)
+    q = torch.zeros(tokens, n_q, 128, dtype=torch.bfloat16, device="cuda")
+    pool = [torch.zeros(blocks, *cases[0][i].shape[1:], dtype=cases[0][i].dtype, device="cuda") for i in (1, 2, 3, 4)]
+    table = torch.zeros(2, width, dtype=torch.int32, device="cuda")
+    plan = ops.PrefillPlan(cases[0][6], cases[0][7], n_q, n_kv, "cuda", min_rows=0, capacity_tokens=tokens, capacity_seqs=2)
+    lse = torch.empty(tokens, n_q, device="cuda")
+    ops.paged_prefill_gqa_fp8(q, *pool, table, plan, cases[0][8], lse_out=lse)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_prefill_gqa_fp8(q, *pool, table, plan, cases[0][8], lse_out=lse)
+    for c in cases + cases[:2]:
+        n = c[6][-1]
+        q[:n].copy_(c[0])
+        for dst, src in zip(pool, c[1:5]):
+            dst[:src.shape[0]].view(torch.uint8).copy_(src.view(torch.uint8))
+        table.zero_()
+        table[:, :c[5].shape[1]].copy_(c[5])
+        out.fill_(3.0)
+        lse.fill_(7.0)
+        plan.refill(c[6], c[7])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert ops.read_status("cuda") == 0
+        if n:
+            _check(out[:n].cpu(), lse[:n].cpu(), *c)
+        assert (out[n:] == 3.0).all() and (lse[n:] == 7.0).all()

@@ -620,6 +620,12 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         tc_fence_before();
         mbar_arrive(&sm.p_full[g]);
       }
+      // A warp without rows is ahead of its group.  It does not enter the next item, where it may have rows and does not
+      // look back, before the group is through with its last tile: a phase of m_ready and p_full gets one arrival a thread.
+      if (idle) {
+        const uint32_t next_own = it + ((it & 1u) == (uint32_t)g ? 0u : 1u);     // the group's next tile
+        if (next_own >= 2) mbar_wait_limited(&sm.p_full[g], ((next_own - 2) >> 1) & 1u, abort_at);
+      }
       // ---- hand the row sums to the convert warps and go on with the next item
       // the references only grow along the tiles: the last tile's is what O is scaled to
       float mm = -INFINITY;

@@ -392,3 +392,25 @@ def test_cut_plans_refilled_and_replayed():
         if n:
             _check(out[:n].cpu(), lse[:n].cpu(), *c)
         assert (out[n:] == 3.0).all() and (lse[n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("max_ctas", [1, 2, 3])
+def test_warps_that_have_rows_again_in_the_next_item(max_ctas):
+    """Items of a few rows between full ones, short and long, odd and even tile counts, one after the other on few CTAs: a
+    warp that only kept the barriers going in one item takes part in the next.  Many runs: the order of arrivals varies."""
+    from auto_infer_b200 import ops
+    q_lens = [3, 128, 1, 128, 33, 128, 64, 2, 128, 5, 97, 128, 1, 1, 128, 40]
+    lens = [900, 128, 130, 300, 400, 1000, 64, 513, 257, 5, 200, 700, 1, 260, 129, 380]
+    c = _case(17, lens, q_lens, 1, 1, 128)
+    first, lse = _run(*c)
+    _check(first, lse, *c)
+    for split in (0, None):
+        plan = ops.PrefillPlan(c[6], c[7], 1, 1, "cuda", min_rows=0, split_ctas=split)
+        dev = [x.cuda() for x in c[:6]]
+        if split is None:
+            first = ops.paged_prefill_gqa_fp8(*dev, plan, c[8]).cpu()
+        for _ in range(30):
+            got = ops.paged_prefill_gqa_fp8(*dev, plan, c[8], max_ctas=max_ctas)
+        assert torch.equal(got.cpu(), first) or split == 0
+        _check(got.cpu(), lse, *c)
+    assert ops.read_status("cuda") == 0

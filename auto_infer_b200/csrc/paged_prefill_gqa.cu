@@ -717,6 +717,7 @@ extern "C" int b200_prefill_plan(const int32_t* cu_q, const int32_t* kv_lens,
   plan[0] = kPfMagic;
   plan[1] = (int32_t)items.size();
   for (int i = 2; i < kPlanHeaderInts; ++i) plan[i] = 0;
+  plan[kHdrHeadGroup] = group;
   if (!items.empty())
     memcpy(plan + kPlanHeaderInts, items.data(), items.size() * sizeof(PrefillItem));
   info->num_items = (int32_t)items.size();

@@ -26,8 +26,8 @@
 // tile of 128 x 128.  A tile takes about 1850 cycles: each group's chain scores -> maximum -> weights -> P is about 3700
 // long, two of them run, and a softmax warp issues an instruction in about three cycles.  Where an item ends, O has
 // to be read before the next item's first P V.  Measured (32 query heads, 8 kv heads): 525 us on an 8192-token prompt (1046
-// TFLOP/s), 106 us on four 512-token chunks over cached prefixes, 41 us on 16 drafts of 5 tokens over 512 to 4096
-// tokens.  Where few items meet many SMs the plan cuts them along the keys (b200_prefill_split) and a second kernel joins
+// TFLOP/s), 106 us on four 512-token chunks over cached prefixes, 38 us on 16 drafts of 5 tokens over 512 to 4096
+// tokens (42 uncut).  Where few items meet many SMs the plan cuts them along the keys (b200_prefill_split) and a second kernel joins
 // the pieces: 81 us instead of 985 on 16 rows over 131072 tokens, 85 instead of 262 on 2 x 64 rows over 32768, 53 instead
 // of 69 on 16 drafts over 2048 to 8192.  What else was tried: both groups on row tiles of their own with one K / V stream (620 us: the
 // instruction footprint of two O rescales), the groups' exponential sections kept apart by a barrier (799 us against 742 at
@@ -469,10 +469,11 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         tc_fence_after();
         if (idle) {                                    // no row of this warp counts: keep the barriers going
           mbar_arrive(&sm.s_empty[sb]);
-          // a phase of m_ready may not get this warp's arrivals of two tiles: the group is through with its previous one
-          if (it >= 2) mbar_wait_limited(&sm.p_full[g], ((it - 2) >> 1) & 1u, abort_at);
           mbar_arrive(&sm.m_ready[it & 1u]);
           mbar_arrive(&sm.p_full[g]);
+          // Not ahead of the group: a phase of m_ready and p_full gets one arrival a thread, also when the warp has rows
+          // again in the next item and does not look back there.
+          mbar_wait_limited(&sm.p_full[g], (it >> 1) & 1u, abort_at);
           continue;
         }
         // Columns past the row's limit become -inf in place, a quarter of the row at a time: few tiles need it, and code
@@ -619,12 +620,6 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sm.p_full[g]);
-      }
-      // A warp without rows is ahead of its group.  It does not enter the next item, where it may have rows and does not
-      // look back, before the group is through with its last tile: a phase of m_ready and p_full gets one arrival a thread.
-      if (idle) {
-        const uint32_t next_own = it + ((it & 1u) == (uint32_t)g ? 0u : 1u);     // the group's next tile
-        if (next_own >= 2) mbar_wait_limited(&sm.p_full[g], ((next_own - 2) >> 1) & 1u, abort_at);
       }
       // ---- hand the row sums to the convert warps and go on with the next item
       // the references only grow along the tiles: the last tile's is what O is scaled to
@@ -957,18 +952,25 @@ extern "C" int b200_prefill_split(int32_t* plan, size_t plan_bytes, int num_ctas
   for (int i = kHdrPieces; i <= kHdrGroups; ++i) plan[i] = 0;
   info->plan_ints = base;
   *num_partials = 0;
-  // What an item or piece costs besides its tiles, and a merge, in tiles (the list is sorted: items[0] is the longest)
-  constexpr float kItemCost = 6.f, kMergeCost = 4.f;
   constexpr int kLeast = 4;                                  // tiles of a piece
-  int64_t total = 0;
-  for (int i = 0; i < n; ++i) total += items[i].n_tiles;
+  int64_t total = 0, all_rows = 0;
+  for (int i = 0; i < n; ++i) {
+    total += items[i].n_tiles;
+    all_rows += std::min(items[i].q_len * plan[kHdrHeadGroup] - items[i].row0, kPfRows);
+  }
   if (n == 0 || total == 0 || n > 4 * num_ctas) return B200_OK;
   const float longest = (float)items[0].n_tiles, share = (float)total / num_ctas, rounds = (float)n / num_ctas;
+  // What an item or piece costs besides its tiles, and the join, in tiles: fitted to steps measured both ways (four
+  // 512-token chunks 122 us cut, 106 whole; three odd sequences 113 and 99; 16 drafts of 20 rows 38 and 42, or 53 and 69
+  // over longer contexts; 2 x 64 rows over 32768 tokens 85 and 262).
+  const float filled = (float)all_rows / ((float)n * kPfRows);
+  const float item_cost = 3.f + 5.f * filled, join_cost = 2.f + 2.f * filled;
   const int per = std::max((int)std::ceil(share), 2 * kLeast);
-  const float whole = rounds <= 1.f ? longest + kItemCost
-                                    : std::min(std::ceil(rounds) * (longest + kItemCost),
-                                               share + longest / 2 + kItemCost * (rounds + 1));
-  const float cut = per + kItemCost * (rounds + 2) + kMergeCost;
+  // the list is sorted: items[0] is the longest
+  const float whole = rounds <= 1.f ? longest + item_cost
+                                    : std::min(std::ceil(rounds) * (longest + item_cost),
+                                               share + longest / 2 + item_cost * (rounds + 1));
+  const float cut = per + item_cost * (rounds + 2) + join_cost;
   if (cut > 0.93f * whole) return B200_OK;
 
   std::vector<PrefillPiece> pieces;

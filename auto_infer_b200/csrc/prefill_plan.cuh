@@ -35,6 +35,7 @@ struct PieceGroup {                           // a cut item: its records lie one
 };
 constexpr int kPieceInts = 12, kPieceGroupInts = 8;
 constexpr int kHdrPieces = 4, kHdrOffPieces = 5, kHdrOffGroups = 6, kHdrGroups = 7;
+constexpr int kHdrHeadGroup = 8;                                // query heads of a kv head
 constexpr int kPieceRecFloats = kPfRows * kPfHeadDim + kPfRows;   // normalised rows, then their log2 sums
 static_assert(sizeof(PrefillPiece) == kPieceInts * 4 && sizeof(PieceGroup) == kPieceGroupInts * 4, "piece layout");
 

@@ -410,6 +410,8 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           PrefillPiece rec;
           if (take_item(item_no, rec) < 0) break;
           const int n_tiles = rec.n_tiles;
+          // Also an item without tiles waits for the O before it to be read: o_done and o_free go item by item.
+          if (n_tiles == 0 && item_no > 0) mbar_wait_limited(&sm.o_free, (item_no - 1) & 1u, abort_at);
 #pragma unroll 1
           for (int tile = 0; tile < n_tiles; ++tile, ++it) {
             const int g = it & 1u;                            // the group that owns this tile, and its V buffer
@@ -469,10 +471,11 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         tc_fence_after();
         if (idle) {                                    // no row of this warp counts: keep the barriers going
           mbar_arrive(&sm.s_empty[sb]);
+          // Never ahead of the group: a phase of m_ready and p_full gets one arrival a thread.  The first wait is for an item
+          // before in which the others had work to do, the second for one behind where this warp has and does not look back.
+          if (it >= 2) mbar_wait_limited(&sm.p_full[g], ((it - 2) >> 1) & 1u, abort_at);
           mbar_arrive(&sm.m_ready[it & 1u]);
           mbar_arrive(&sm.p_full[g]);
-          // Not ahead of the group: a phase of m_ready and p_full gets one arrival a thread, also when the warp has rows
-          // again in the next item and does not look back there.
           mbar_wait_limited(&sm.p_full[g], (it >> 1) & 1u, abort_at);
           continue;
         }

@@ -414,3 +414,28 @@ def test_warps_that_have_rows_again_in_the_next_item(max_ctas):
         assert torch.equal(got.cpu(), first) or split == 0
         _check(got.cpu(), lse, *c)
     assert ops.read_status("cuda") == 0
+
+
+def test_few_and_many_rows_in_turn_many_times():
+    """Pieces and items of 1 to 130 rows follow one another on a CTA in ever new orders: the same bits every time, on any
+    number of CTAs, and no wait runs out - also with items that have no tile at all (more queries than keys)."""
+    from auto_infer_b200 import ops
+    for q_lens, lens, n_q, n_kv, bs in (([33, 64, 130, 1, 100, 1, 3], [129, 129, 6000, 1000, 500, 50, 1000], 8, 8, 256),
+                                        ([128, 300, 2, 3, 300, 17, 2], [3000, 300, 6000, 3000, 300, 3000, 128], 32, 8, 16),
+                                        ([300, 130, 33, 300, 64, 1], [300, 1, 50, 500, 128, 1], 16, 2, 16),
+                                        ([300, 33, 17, 300, 3, 100], [128, 128, 6000, 300, 3, 6000], 32, 8, 128)):
+        c = _case(len(q_lens), lens, q_lens, n_q, n_kv, bs)
+        dev = [x.cuda() for x in c[:6]]
+        plan = ops.PrefillPlan(c[6], c[7], n_q, n_kv, "cuda", min_rows=0)
+        whole = ops.PrefillPlan(c[6], c[7], n_q, n_kv, "cuda", min_rows=0, split_ctas=0)
+        for x in (plan, whole):
+            want = None
+            for k in range(120):
+                lse = torch.empty(c[6][-1], n_q, device="cuda")
+                got = ops.paged_prefill_gqa_fp8(*dev, x, c[8], lse_out=lse, max_ctas=(0, 50, 3, 20, 1)[k % 5], out_f32=True)
+                if want is None:
+                    want = got, lse
+                assert torch.equal(got, want[0]) and torch.equal(lse, want[1]), k
+            assert ops.read_status("cuda") == 0
+        out, sums = _run(*c)
+        _check(out, sums, *c)

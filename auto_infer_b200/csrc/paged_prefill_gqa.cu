@@ -390,13 +390,13 @@ paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap k_map,
         PrefillItem rec;
         if (take_item(item_no, rec) < 0) break;
         const int n_tiles = rec.n_tiles;
+        // The previous item's O has been read.  Also an item without tiles waits: o_done and o_free go item by item.
+        if (item_no > 0) mbar_wait_bounded(&sm.o_free, (item_no - 1) & 1u, abort_flag, p.status);
         for (int tile = 0; tile < n_tiles; ++tile, ++it) {
           const int s = it % kTcVStages;
           const int g = it & 1u;                            // the group that owns this tile
           mbar_wait_bounded(&sm.v_full[s], (it / kTcVStages) & 1u, abort_flag, p.status);
           mbar_wait_bounded(&sm.p_full[g], (it >> 1) & 1u, abort_flag, p.status);
-          if (tile == 0 && item_no > 0)                     // the previous item's O has been read
-            mbar_wait_bounded(&sm.o_free, (item_no - 1) & 1u, abort_flag, p.status);
           tc_fence_after();
           PF_TRACE(5, it);
           const uint32_t v_lo = dv_lo + (uint32_t)((s * kPfTileBytes) >> 4);

@@ -439,3 +439,25 @@ def test_few_and_many_rows_in_turn_many_times():
             assert ops.read_status("cuda") == 0
         out, sums = _run(*c)
         _check(out, sums, *c)
+
+
+@pytest.mark.parametrize("max_ctas", [1, 3, 0])
+def test_many_items_without_keys(max_ctas):
+    """More queries than keys: item after item that sees nothing comes out as zeros with lse = -inf, the others beside them
+    are not disturbed; the kernel over a 16-bit cache has the same queue."""
+    from auto_infer_b200 import ops
+    c = _case(44, [1, 300, 0, 2], [700, 300, 260, 1], 8, 2, 16)
+    dev = [x.cuda() for x in c[:6]]
+    plan = ops.PrefillPlan(c[6], c[7], 8, 2, "cuda", min_rows=0)
+    want, want_lse = attention(*c)
+    empty = want_lse == -math.inf
+    kc = (dev[1].float() * dev[3][:, None, :, None]).to(torch.bfloat16)
+    vc = (dev[2].float() * dev[4][:, None, :, None]).to(torch.bfloat16)
+    for _ in range(20):
+        for call in (lambda **kw: ops.paged_prefill_gqa_fp8(*dev, plan, c[8], **kw),
+                     lambda **kw: ops.paged_prefill_gqa(dev[0], kc, vc, dev[5], plan, c[8], **kw)):
+            lse = torch.full(want_lse.shape, 7.0, device="cuda")
+            got = call(lse_out=lse, max_ctas=max_ctas, out=torch.full(want.shape, 3.0, device="cuda"))
+            assert torch.equal(lse.cpu() == -math.inf, empty) and (got.cpu()[empty] == 0).all()
+            assert (got.cpu().double() - want).abs().max() <= 2.0 ** -5 * want.abs().max()    # bf16 K, V and weights
+    assert ops.read_status("cuda") == 0

@@ -25,7 +25,7 @@
 // Tensor-bound: flops = 4 * 128 * sum over rows of visible keys; 1024 tensor cycles and 1024 cycles of exponentials for a
 // tile of 128 x 128.  A tile takes about 1850 cycles: each group's chain scores -> maximum -> weights -> P is about 3700
 // long, two of them run, and a softmax warp issues an instruction in about three cycles.  Where an item ends, O has
-// to be read before the next item's first P V.  Measured (32 query heads, 8 kv heads): 525 us on an 8192-token prompt (1046
+// to be read before the next item's first P V.  Measured (32 query heads, 8 kv heads): 520 us on an 8192-token prompt (1057
 // TFLOP/s), 106 us on four 512-token chunks over cached prefixes, 38 us on 16 drafts of 5 tokens over 512 to 4096
 // tokens (42 uncut).  Where few items meet many SMs the plan cuts them along the keys (b200_prefill_split) and a second kernel joins
 // the pieces: 81 us instead of 985 on 16 rows over 131072 tokens, 85 instead of 262 on 2 x 64 rows over 32768, 53 instead
@@ -174,7 +174,7 @@ __device__ __forceinline__ void umma_f8_ss_lo(uint32_t tmem_d, uint32_t a_lo, ui
       ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(kAccumulate ? 1 : 0));
 }
 // kOnePage: pages of 128 tokens or more, one pair of scales per tile.  kCut: a plan that has pieces, or that a recorded
-// launch may find them in (545 us instead of 525 on an 8192-token prompt without any: the roles that walk tiles have no
+// launch may find them in (4 % slower on an 8192-token prompt without any: the roles that walk tiles have no
 // register left for where a piece begins).
 template <bool kOnePage, bool kCut>
 __global__ void __launch_bounds__(kP8Threads, 1)
@@ -410,15 +410,13 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           PrefillPiece rec;
           if (take_item(item_no, rec) < 0) break;
           const int n_tiles = rec.n_tiles;
-          // Also an item without tiles waits for the O before it to be read: o_done and o_free go item by item.
-          if (n_tiles == 0 && item_no > 0) mbar_wait_limited(&sm.o_free, (item_no - 1) & 1u, abort_at);
+          // The previous item's O has been read.  Also an item without tiles waits: o_done and o_free go item by item.
+          if (item_no > 0) mbar_wait_limited(&sm.o_free, (item_no - 1) & 1u, abort_at);
 #pragma unroll 1
           for (int tile = 0; tile < n_tiles; ++tile, ++it) {
             const int g = it & 1u;                            // the group that owns this tile, and its V buffer
             mbar_wait_limited(&sm.v16_full[g], (it >> 1) & 1u, abort_at);
             mbar_wait_limited(&sm.p_full[g], (it >> 1) & 1u, abort_at);
-            if (tile == 0 && item_no > 0)                     // the previous item's O has been read
-              mbar_wait_limited(&sm.o_free, (item_no - 1) & 1u, abort_at);
             tc_fence_after();
             const uint32_t v_lo = dv_lo + (uint32_t)((g * 2 * kP8TileBytes) >> 4);
             const uint32_t p_tmem = tmem + kP8PCol + g * 64;  // P of the tile: 128 tokens as f16 pairs

@@ -73,7 +73,7 @@ struct __align__(1024) Prefill8Smem {
   uint8_t k[kP8KStages][kP8TileBytes];     // [128 tokens][128 B], swizzled
   uint8_t v[kP8VStages][kP8TileBytes];
   uint8_t v16[2][2 * kP8TileBytes];        // f16: [dims 0-63 | dims 64-127], 128 tokens x 128 B each, swizzled
-  float row_factor[2][kPfRows];            // per item parity: softmax scale * log2(e) * 2^-u of the row
+  float row_factor[2][kPfRows];            // per item parity: |softmax scale| * log2(e) * 2^-u of the row
   float row_l[2][kPfRows];                 // end of item: the groups' row sums
   float row_m[2][kPfRows];                 // and the maxima they refer to
   float row_mfin[kPfRows];                 // end of item: the reference of O
@@ -686,8 +686,10 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       }
       // exponent field of the largest; 8 and more: both factors are normal
       const int e = max((int)(max(top & 0xffffu, top >> 16) >> 7), 8);
-      up = e == 255 ? NAN : __uint_as_float((uint32_t)(261 - e) << 23);   // 2^(7 - (e - 127)); any inf or NaN: the row is NaN
-      row_factor = __uint_as_float((uint32_t)(e - 7) << 23) * p.scale_log2;
+      // 2^(7 - (e - 127)) with the sign of the softmax scale, so that the factor behind the product is not negative: the
+      // softmax threads take the maximum of a row, and mask it, before they multiply.  Any inf or NaN: the row is NaN.
+      up = e == 255 ? NAN : copysignf(__uint_as_float((uint32_t)(261 - e) << 23), p.scale_log2);
+      row_factor = __uint_as_float((uint32_t)(e - 7) << 23) * fabsf(p.scale_log2);
       return Row{x.n_tiles, x.kv_len - first_of(x) * kPfTile, kCut ? x.partial : -1, valid ? tok * p.num_q_heads + head : -1};
     };
     auto put_step = [&](uint32_t k) {

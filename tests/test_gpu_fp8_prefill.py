@@ -461,3 +461,20 @@ def test_many_items_without_keys(max_ctas):
             assert torch.equal(lse.cpu() == -math.inf, empty) and (got.cpu()[empty] == 0).all()
             assert (got.cpu().double() - want).abs().max() <= 2.0 ** -5 * want.abs().max()    # bf16 K, V and weights
     assert ops.read_status("cuda") == 0
+
+
+@pytest.mark.parametrize("bs", [32, 128])
+@pytest.mark.parametrize("scale", [-128 ** -0.5, -0.01, -1.0, 0.0])
+def test_softmax_scales_that_are_negative_or_zero(scale, bs):
+    """The largest score then belongs to the smallest product, and the masked keys stay the smallest: whole items and cut
+    ones, and the form for few rows."""
+    from auto_infer_b200 import ops
+    for lens, q_lens in (([130, 300, 17], [130, 45, 17]), ([5000], [7])):
+        c = (*_case(21, lens, q_lens, 8, 2, bs, q_mul=0.5)[:8], scale)
+        _check(*_run(*c), *c)
+        _check(*_run(*c, out_f32=True), *c)
+    c = (*_case(22, [333, 64], [2, 1], 8, 2, bs, q_mul=0.5)[:8], scale)
+    plan = ops.DecodePlan(c[6], c[7], 8, 2, "cuda")
+    lse = torch.empty(3, 8, device="cuda")
+    got = ops.paged_decode_gqa_fp8(*[x.cuda() for x in c[:6]], plan, scale, lse_out=lse)
+    _check(got.cpu(), lse.cpu(), *c)

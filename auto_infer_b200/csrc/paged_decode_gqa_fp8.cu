@@ -14,13 +14,15 @@
 //     9 to 16 rows take two column tiles.
 //   * codes become f16 on their way from shared memory to the MMA: e4m3 -> f16 is exact and one instruction per
 //     pair.  Q (bf16) is scaled per row by a power of two so that it fits f16 exactly, and the weights P are f16
-//     too, three bits more than bf16.  (The e4m3 form of mma.sync converts in the same way on this part: 20 cycles a
+//     too, three bits more than bf16 over the range that counts (below).  (The e4m3 form of mma.sync converts in the same way on this part: 20 cycles a
 //     scheduler for 32 x 8 codes, two f16 MMAs take 16.)
 //   * no element is multiplied by a scale.  K's scale is uniform over 16 tokens (the least a page holds) and goes
 //     into the factor that turns a product into a log2 score.  V's scale goes into the weight,
 //     w = 2^(x + log2 s_v - M): M is the running maximum of x + log2 s_v, kept beside the running maximum m of
-//     the scores x that the row sum l refers to.  So w <= 1 whatever the pages' scales are, and the largest
-//     contributions have the most bits.  O is in units of 2^M and is brought to l's 2^m when the row is written.
+//     the scores x that the row sum l refers to, and the P of the product is 2^15 w.  So P fits f16 whatever the pages'
+//     scales are, the largest contributions have the most bits, and those down to 2^-29 of them lose none: many small
+//     weights beside one key that carries the row (and may have a V of zeros) add up to what they should.  O is in units
+//     of 2^(M - 15) and is brought to l's 2^m when the row is written.
 //   * M only has to be common to the eight lanes that hold a row; a vote finds the tiles that raise it, all others
 //     pass without a shuffle.  m is each lane's own until the end.
 //   * the order of the 16 dims of a k-step, and which column of V an O^T row stands for, are free as long as both
@@ -49,6 +51,9 @@ constexpr int kF8TileBytes = kTileTokens * kFp8HeadDim;          // K or V tile:
 constexpr int kF8StageBytes = 2 * kF8TileBytes;
 constexpr int kF8MaxBoxes = kTileTokens / kFp8MinBlockSize;      // pages a tile can span
 constexpr int kF8SlotFloats = kMaxRows * kHeadDim;
+// O's reference lies 2^15 below the largest contribution so far: the largest weight is 2^15, f16 ends at 2^16, and what
+// a weight keeps of its bits does not begin to shrink before it is 2^-29 of the largest (2^-14 without).
+constexpr float kF8WeightLog2 = 15.f;
 static_assert(kF8GroupWarps * 32 == kTileTokens && kF8Warps == 8, "the merge is written for eight warps");
 static_assert(kHeadDim == kFp8HeadDim, "one head width");
 
@@ -193,7 +198,7 @@ __device__ __forceinline__ void attend_tile(RowState<kN>& st, const uint32_t (&q
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const float ms = st.m[n][e] == -INFINITY ? 0.f : st.m[n][e];
-      const float os = st.mo[n][e] == -INFINITY ? 0.f : st.mo[n][e];
+      const float os = st.mo[n][e] == -INFINITY ? 0.f : st.mo[n][e] - kF8WeightLog2;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         // w = p 2^up with p = 2^(x - m); bounded, so that a weight whose p is 0 does not become 0 * inf
@@ -675,10 +680,10 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         go = fmaxf(go, sm.red_o[ww][row]);
         lsum += sm.red_l[ww][row];
       }
-      // O is in units of 2^go, the sum in units of 2^g; the factor between them in two halves, each of
+      // O is in units of 2^(go - 15), the sum in units of 2^g; the factor between them in two halves, each of
       // which fp32 holds however far apart they are
       inv_r[h] = lsum == 0.f ? 0.f : 1.f / lsum;          // a NaN sum stays one
-      unit_r[h] = go == -INFINITY ? 0.f : fast_exp2((go - g) * 0.5f);
+      unit_r[h] = go == -INFINITY ? 0.f : fast_exp2((go - kF8WeightLog2 - g) * 0.5f);
       lse_r[h] = lsum == 0.f ? -INFINITY : g * 0.6931471805599453f + __logf(lsum);
     }
     named_bar_sync(1, kF8Consumers);                           // (3) the four slots hold the warp-pair sums

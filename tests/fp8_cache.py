@@ -1,4 +1,6 @@
 """Test helper: 8-bit paged caches with shuffled pages, and their values in 64 bits."""
+import math
+
 import torch
 
 from oracle import paged_attention_oracle as orc
@@ -102,4 +104,31 @@ def smallest_weights(q, kc, vc, ks, vs, table, cu, kv_lens, scale, causal_base=N
     return out
 
 
-__all__ = ["smallest_weights", "E4M3", "as_values", "empty_pool", "random_pool", "deal_pages", "attention", "orc"]
+def sink_case(seed, lens, q_lens, n_q, bs, mass, sink_v):
+    """Rows whose first key takes the share ``mass`` of the softmax over a long context and has a V of ``sink_v`` times
+    the others' size (0: of zeros), so that the row's output is made of many weights, each far below that key's.  One kv
+    head; half of V's columns are of one sign.  Same tuple as the kernel tests' cases."""
+    g = torch.Generator().manual_seed(seed)
+    blocks, table, _ = deal_pages(g, lens, bs)
+    kc, ks = random_pool(g, blocks, bs, 1, spread=0.0)
+    vc, vs = random_pool(g, blocks, bs, 1, spread=0.0)
+    kx, vx = kc.float(), vc.float()
+    kx[..., 0] = 0.0
+    vx[..., ::2] = vx[..., ::2].abs()
+    for b in range(len(lens)):
+        page = int(table[b, 0])
+        kx[page, 0] = 0.0
+        kx[page, 0, 0, 0] = 448.0
+        vx[page, 0] *= sink_v
+    cu = torch.tensor(q_lens).cumsum(0).tolist()
+    q = torch.randn(cu[-1], n_q, 128, generator=g)
+    scale, at = 128 ** -0.5, 0
+    for n, end in zip(lens, cu):
+        # the other scores are about N(0, 1): their sum is about n exp(1/2)
+        gap = math.log(mass / (1 - mass)) + math.log(max(n - 1, 1)) + 0.5
+        q[at:end, :, 0] = gap / (scale * 448.0 * float(ks[0, 0]))
+        at = end
+    return q.to(torch.bfloat16), kx.to(E4M3), vx.to(E4M3), ks, vs, table, cu, list(lens), scale
+
+
+__all__ = ["sink_case", "smallest_weights", "E4M3", "as_values", "empty_pool", "random_pool", "deal_pages", "attention", "orc"]

@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from tests.fp8_cache import attention, deal_pages, random_pool, smallest_weights
+from tests.fp8_cache import attention, deal_pages, random_pool, sink_case, smallest_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -317,3 +317,20 @@ def test_plans_of_another_kind_are_refused():
         for plan in plans:
             with pytest.raises(ValueError, match="the plan must be"):
                 call(*dev, plan, c[8])
+
+
+@pytest.mark.parametrize("mass", [0.9, 0.99, 0.999])
+@pytest.mark.parametrize("sink_v", [0.0, 0.005])
+@pytest.mark.parametrize("n, q_len, num_ctas", [(131072, 1, 1), (131072, 2, 148), (9000, 1, 2)])
+def test_many_small_weights_beside_a_key_that_carries_the_row(mass, sink_v, n, q_len, num_ctas):
+    """Tolerance: the largest P of a row is 2^15 at least of the reference ``smallest_weights`` takes as 1, so what it derives for
+    weights below f16's normal range is 2^-15 of it.  O is summed over n / 16 steps of the product in fp32, each off by
+    2^-24 of the sum so far at most; the rest as above."""
+    c = sink_case(41, [n], [q_len], 8, 16 if n < 10000 else 128, mass, sink_v)
+    got, lse = _run(*c, num_ctas=num_ctas, out_f32=True)
+    want, want_lse = attention(*c)
+    a = _magnitude(*c)
+    tol = (2.0 ** -11 + 2.0 ** -16 + n / 16 * 2.0 ** -24) * a + 2.0 ** -15 * smallest_weights(*c)
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+    torch.testing.assert_close(lse.double(), want_lse, rtol=2.0 ** -18, atol=2.0 ** -16)

@@ -15,11 +15,13 @@
 //   and shared-memory time and K half of the loads.
 // * V is converted to f16 (exact) by the warpgroup that also writes O: splitting P like Q would cost the
 //   softmax threads, which set the pace, five instructions per pair of weights, while that warpgroup idles
-//   between items.  P is f16, three more bits than bf16.
+//   between items.  P is f16, three more bits than bf16 over the range that counts (below).
 // * No element is multiplied by a scale.  K's scale and the row's 2^-u are in the factor that
-//   turns a product into a log2 score; V's scale is in the weight, w = 2^(x + log2 s_v - M) with M the running
-//   maximum of x + log2 s_v (handed between the groups with O), while each group's row sum refers to its own
-//   running maximum m of x.  A page is at least 16 tokens: a tile has 8 column groups of 16, each with its
+//   turns a product into a log2 score; V's scale is in the weight, w = 2^(x + log2 s_v - M) with M 7 below the running
+//   maximum of x + log2 s_v (handed between the groups with O; taken late, so that w stays under 2^15), while each group's
+//   row sum refers to its own running maximum m of x.  Weights lose no bits of f16 down to 2^-21 of the largest and are not
+//   dropped down to 2^-32: many small ones beside a key that carries the row (and may have a V of zeros) add up to
+//   what they should.  A page is at least 16 tokens: a tile has 8 column groups of 16, each with its
 //   scales, or one pair for the whole tile when pages hold 128 tokens or more.
 //
 // Tensor-bound: flops = 4 * 128 * sum over rows of visible keys; 1024 tensor cycles and 1024 cycles of exponentials for a
@@ -65,6 +67,11 @@ struct P8Regs {
   static constexpr int kSoftmax = kOnePage ? 184 : 192, kOther = kOnePage ? 56 : 48, kConvert = kOnePage ? 88 : 80;
 };
 constexpr int kP8TmemCols = 512;          // S0 [0,128) S1 [128,256) O [256,384) P_A [384,448) P_B [448,512)
+// O is rescaled when a row's largest contribution outgrows what it was when the reference was taken by 2^kP8Lazy, and the
+// reference is taken 2^kP8Lift below it: the largest weight is 2^15, f16 ends at 2^16, and a weight loses none of its bits
+// down to 2^-21 of the largest contribution.  More lift for less laziness costs rescales: an 8192-token prompt takes 522 us
+// with 8 and 7, 535 with 6 and 9, 549 with 4 and 11.
+constexpr float kP8Lazy = 8.f, kP8Lift = 15.f - kP8Lazy;
 constexpr int kP8OCol = 256;
 constexpr int kP8PCol = 384;
 
@@ -530,7 +537,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                             __uint_as_float(sv[u >> 1][(u & 1) * 16 + c + 1]));
           if constexpr (kOnePage) {
             mx = fmaxf(fmax3(mq[0], mq[1], mq[2]), fmax3(fmax3(mq[3], mq[4], mq[5]), mq[6], mq[7])) * f[0];
-            my = mx + lv[0];
+            my = mx + (lv[0] - kP8Lift);
           } else {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
@@ -538,10 +545,11 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
               mx = fmaxf(mx, x);
               my = fmaxf(my, x + lv[u]);
             }
+            my -= kP8Lift;
           }
         }
-        // lazy rescale: only when some row of the warp outgrew the stale reference by 2^8
-        const bool grow = my - m_in > 8.f || (m_in == -INFINITY && my > -INFINITY);
+        // lazy rescale: only when some row of the warp outgrew the stale reference
+        const bool grow = my - m_in > kP8Lazy || (m_in == -INFINITY && my > -INFINITY);
         const bool rescale = __any_sync(0xffffffffu, grow);
         const float m_used = rescale ? fmaxf(m_in, my) : m_in;
         sm.row_ms[it & 1u][r] = m_used;
@@ -804,7 +812,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
                                            : __fadd_rn(__fmul_rn(sm.row_l[0][r], fast_exp2(m0 - mm)),
                                                        __fmul_rn(sm.row_l[1][r], fast_exp2(m1 - mm)));
         mbar_arrive(&sm.l_empty);
-        // O is in units of 2^mo, the sum in units of 2^mm; the factor between them in two halves, each of
+        // O is in units of 2^(mo - kP8Lift), the sum in units of 2^mm; the factor between them in two halves, each of
         // which fp32 holds however far apart they are
         const float half_unit = fast_exp2((mo - (mm == -INFINITY ? 0.f : mm)) * 0.5f);
         const float inv = half_unit / lsum;

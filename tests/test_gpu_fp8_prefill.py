@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from tests.fp8_cache import attention, deal_pages, random_pool, smallest_weights
+from tests.fp8_cache import attention, deal_pages, random_pool, sink_case, smallest_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -478,3 +478,24 @@ def test_softmax_scales_that_are_negative_or_zero(scale, bs):
     lse = torch.empty(3, 8, device="cuda")
     got = ops.paged_decode_gqa_fp8(*[x.cuda() for x in c[:6]], plan, scale, lse_out=lse)
     _check(got.cpu(), lse.cpu(), *c)
+
+
+@pytest.mark.parametrize("mass", [0.9, 0.99, 0.999])
+@pytest.mark.parametrize("sink_v", [0.0, 0.005])
+@pytest.mark.parametrize("n, q_len, bs, split", [(131072, 3, 128, 0), (131072, 3, 128, None), (9000, 20, 16, 0), (9000, 20, 128, 0)])
+def test_many_small_weights_beside_a_key_that_carries_the_row(mass, sink_v, n, q_len, bs, split):
+    """Tolerance: a row's largest weight is 2^7 at least of the reference that ``smallest_weights`` takes as 1, so what it derives
+    for weights below f16's normal range is 2^-7 of it.  O is summed over n / 16 steps of the product in fp32, each
+    off by 2^-24 of the sum so far at most; the rest as above."""
+    from auto_infer_b200 import ops
+    c = sink_case(43, [n], [q_len], 8, bs, mass, sink_v)
+    plan = ops.PrefillPlan(c[6], c[7], 8, 1, "cuda", min_rows=0, split_ctas=split)
+    lse = torch.empty(q_len, 8, device="cuda")
+    got = ops.paged_prefill_gqa_fp8(*[x.cuda() for x in c[:6]], plan, c[8], lse_out=lse, out_f32=True).cpu()
+    assert ops.read_status("cuda") == 0
+    want, want_lse = attention(*c)
+    a = attention(c[0], c[1], c[2].float().abs().to(c[2].dtype), *c[3:])[0]
+    tol = (2.0 ** -11 + 2.0 ** -13 + 2.0 ** -16 + n / 16 * 2.0 ** -24) * a + 2.0 ** -7 * smallest_weights(*c)
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+    torch.testing.assert_close(lse.cpu().double(), want_lse, rtol=2.0 ** -16, atol=2.0 ** -14)

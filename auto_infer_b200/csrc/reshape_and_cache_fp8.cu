@@ -255,7 +255,8 @@ reshape_and_cache_fp8_kernel(const QuantWriteParams p) {
           top = __reduce_max_sync(0xffffffffu, larger_half(top));
         }
         const PageScale ps(top, s_old, token_of[0] >= 0, plain);
-        if (lane == 0) *scale_at = ps.s;           // the warp has read it: the reduction above waited for all lanes
+        __syncwarp();                              // all lanes have read the old scale: a reduction orders no memory
+        if (lane == 0) *scale_at = ps.s;
         uint8_t* const rows_at = (is_v ? p.cache[1] : p.cache[0]) +
                                  ((int64_t)page * p.block_size * p.num_kv_heads + head) * kFp8HeadDim + part * 8;
         const int64_t row_bytes = (int64_t)p.num_kv_heads * kFp8HeadDim;

@@ -226,3 +226,24 @@ def test_slots_of_64_bits_do_not_wrap_into_the_pool():
     assert ops.read_status("cuda") == 1              # the first is past the pool, the second a padding row
     written = kc.view(torch.uint8).view(32, -1).any(-1).nonzero().flatten().tolist()
     assert written == [7]
+
+
+@pytest.mark.parametrize("n_kv, bs", [(8, 128), (3, 16)])
+def test_scales_that_grow_call_after_call(n_kv, bs):
+    """Two hundred decode rows, each into a page of its own, larger call after call: every lane of a page's warp goes by the scale
+    that was there before one of them replaced it."""
+    from auto_infer_b200 import ops
+    g = torch.Generator().manual_seed(12)
+    pages = 200
+    pools = [random_pool(g, pages, bs, n_kv, spread=1.0) for _ in range(2)]
+    (kc, ks), (vc, vs) = [[x.cuda() for x in pool] for pool in pools]
+    wants = [(as_values(codes), scale.double()) for codes, scale in pools]
+    for call in range(8):
+        rows = [(_rows(g, pages, n_kv, 0.3).float() * 2.5 ** call).to(torch.bfloat16) for _ in range(2)]
+        slots = torch.arange(pages) * bs + 1 + call
+        ops.reshape_and_cache_fp8(rows[0].cuda(), rows[1].cuda(), kc, vc, ks, vs, slots.cuda())
+        for x, (want, want_scale), codes, scale in zip(rows, wants, (kc, vc), (ks, vs)):
+            orc.write_kv_fp8(x, want, want_scale, slots.tolist())
+            assert torch.equal(scale.cpu().double(), want_scale), call
+            assert torch.equal(as_values(codes), want), call
+    assert ops.read_status("cuda") == 0

@@ -209,7 +209,8 @@ class B200GraphGqaBackend(B200GqaBackend):
               ctx) -> torch.Tensor:
         if not self.capturing:
             return super()._attn(layer_idx, q, k, v, ctx)
-        meta = cached_step_metadata(ctx, self.n_q_heads, self.n_kv_heads, self.head_dim, q.device)
+        meta = cached_step_metadata(ctx, self.n_q_heads, self.n_kv_heads, self.head_dim, q.device,
+                                    self._kv_elem_bytes)
         if meta is None or not meta.decode.replayable:
             raise RuntimeError(
                 "capture needs one eager step with the same context first (capturing False): the "

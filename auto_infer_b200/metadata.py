@@ -159,19 +159,25 @@ class StepMetadata:
         return self
 
 
-def cached_step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int, device):
-    """The metadata already attached to ``ctx`` for this head geometry, or None."""
+def _step_key(num_q_heads: int, num_kv_heads: int, head_dim: int, device, kv_elem_bytes: int) -> tuple:
+    """What a step's plans depend on besides its lengths: the head geometry, and the size of a cache element (the rates of
+    a mixed step, and whether long items are cut)."""
+    return num_q_heads, num_kv_heads, head_dim, str(device), kv_elem_bytes
+
+
+def cached_step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int, device, kv_elem_bytes: int = 2):
+    """The metadata already attached to ``ctx`` for this head geometry and cache element size, or None."""
     cache = getattr(ctx, _ATTR, None)
     if cache is None:
         return None
-    return cache.get((num_q_heads, num_kv_heads, head_dim, str(device)))
+    return cache.get(_step_key(num_q_heads, num_kv_heads, head_dim, device, kv_elem_bytes))
 
 
 def step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int, device,
                   causal_base: Optional[Sequence[int]] = None, pool: Optional[dict] = None,
                   split_mixed: bool = False, kv_elem_bytes: int = 2) -> StepMetadata:
     """Fetch (or build and attach) the metadata of ``ctx`` for this head
-    geometry.  The context is a plain mutable dataclass in the reference
+    geometry and cache element size.  The context is a plain mutable dataclass in the reference
     (auto_infer/forward_context.py:9), which already carries per-step extras
     such as the rope tables the same way (auto_infer/models/base.py:75).
 
@@ -187,7 +193,7 @@ def step_metadata(ctx, num_q_heads: int, num_kv_heads: int, head_dim: int, devic
     if cache is None:
         cache = {}
         setattr(ctx, _ATTR, cache)
-    key = (num_q_heads, num_kv_heads, head_dim, str(device))
+    key = _step_key(num_q_heads, num_kv_heads, head_dim, device, kv_elem_bytes)
     meta = cache.get(key)
     if meta is None:
         prefill_ctas = 0

@@ -244,3 +244,29 @@ def test_split_refusals(lib):
     assert lib.b200_prefill_split(None, *args[1:]) == -1 and lib.b200_prefill_split(*args[:2], 0, *args[3:]) == -1
     assert lib.b200_prefill_split(*args[:2], 5000, *args[3:]) == -1
     assert lib.b200_prefill_split_bytes(-1, 4) == 0 and lib.b200_prefill_split_workspace_bytes(-1) == 0
+
+
+def test_backends_over_different_caches_do_not_share_a_contexts_plans(monkeypatch):
+    """A 16-bit and an 8-bit backend of one head geometry on one context: a plan for each, whichever comes first."""
+    from auto_infer_b200 import metadata
+    built = []
+
+    class Plans:
+        capacity_seqs = 16
+
+        def __init__(self, *args, split_prefill=False, **kw):
+            self.split_prefill = split_prefill
+            built.append(self)
+
+    monkeypatch.setattr(metadata, "StepMetadata", Plans)
+    for order in ((2, 1), (1, 2)):
+        built.clear()
+        ctx, pools = SimpleNamespace(cu_seqlens_q=[3, 20], seqlens_kv=[50, 40]), {1: {}, 2: {}}
+        got = {n: metadata.step_metadata(ctx, 8, 2, 128, "cpu", pool=pools[n], kv_elem_bytes=n) for n in order}
+        assert got[1].split_prefill and not got[2].split_prefill and len(built) == 2
+        for n in order:
+            assert metadata.step_metadata(ctx, 8, 2, 128, "cpu", pool=pools[n], kv_elem_bytes=n) is got[n]
+            assert metadata.cached_step_metadata(ctx, 8, 2, 128, "cpu", n) is got[n]
+            assert list(pools[n].values()) == [got[n]]
+        assert metadata.cached_step_metadata(ctx, 8, 2, 128, "cpu") is got[2]
+        assert len(built) == 2

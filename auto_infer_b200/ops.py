@@ -556,8 +556,10 @@ class PrefillPlan:
     on the step, so a CUDA graph that recorded it serves later steps.
 
     Where the items are few, long ones are cut along the keys for the kernel over an 8-bit cache
-    (``paged_prefill_gqa_fp8``); ``split_ctas`` is the number of SMs its launch will have (default
-    all of the device, 0: never cut).  The plan owns the workspace of the partial results."""
+    (``paged_prefill_gqa_fp8``; the one over a 16-bit cache reads the uncut items).  ``split_ctas`` is the number of
+    SMs its launch will have, and a plan that is given one is cut from the start; the default is all of the device
+    from the first launch over an 8-bit cache on, 0: never.  The plan owns the workspace of the partial results,
+    which is allocated when a launch first needs it."""
 
     def __init__(self, cu_seqlens_q: Sequence[int], seqlens_kv: Sequence[int], num_q_heads: int,
                  num_kv_heads: int, device, min_rows: int = 16,
@@ -576,6 +578,8 @@ class PrefillPlan:
         self._nbytes = max(lib.b200_prefill_plan_bytes(self.capacity_seqs, self.capacity_tokens, num_q_heads,
                                                        num_kv_heads), 64)
         self._split_ctas = sm_count(self.device) if split_ctas is None else int(split_ctas)
+        self._cutting = bool(split_ctas)
+        self._workspace = None
         if self._split_ctas:
             self._nbytes += lib.b200_prefill_split_bytes(self._nbytes // 32, self._split_ctas)   # an item has 32 bytes
         self._hosts = [torch.empty(self._nbytes // 4, dtype=torch.int32, pin_memory=True)
@@ -586,12 +590,51 @@ class PrefillPlan:
         self.info = PrefillPlanInfo()
         self._build(cu_seqlens_q, seqlens_kv, causal_base)
         used = max(int(self.info.plan_ints), 16)
-        self.dev = torch.zeros(self._nbytes // 4 if self.replayable else used, dtype=torch.int32,
+        self.dev = torch.zeros(self._nbytes // 4 if self.replayable or self._split_ctas else used, dtype=torch.int32,
                                device=self.device)
         self._upload(used)
-        records = 2 * self._split_ctas if self.replayable else self._num_partials
-        self.workspace = torch.empty(lib.b200_prefill_split_workspace_bytes(records), dtype=torch.uint8,
-                                     device=self.device) if records else None
+
+    def _cut(self) -> None:
+        """Cut the step in the host buffer."""
+        partials = ctypes.c_int(0)
+        rc = _lib.load().b200_prefill_split(self.host.data_ptr(), self.host.numel() * 4, self._split_ctas,
+                                            ctypes.byref(self.info), ctypes.byref(partials))
+        _lib.check(rc, "b200_prefill_split")
+        self._num_partials = partials.value
+
+    def _start_cutting(self) -> None:
+        """This step too is cut, unless its launch is being recorded (the upload would be replayed with it)."""
+        self._cutting = True
+        if not torch.cuda.is_current_stream_capturing():
+            self._cut()
+            if self._num_partials:
+                self._upload(int(self.info.plan_ints))
+
+    @property
+    def workspace(self) -> Optional[torch.Tensor]:
+        """Room for the partial results of this step's cut items; None when none is cut."""
+        if self._split_ctas and not self._cutting:
+            self._start_cutting()
+        return self._workspace_of(self._num_partials)
+
+    def _workspace_of(self, records: int) -> Optional[torch.Tensor]:
+        if not records:
+            return None
+        nbytes = _lib.load().b200_prefill_split_workspace_bytes(records)
+        if self._workspace is None or self._workspace.numel() < nbytes:
+            self._workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return self._workspace
+
+    def _launch_workspace(self) -> Optional[torch.Tensor]:
+        """The workspace of a launch over an 8-bit cache: of a replayable plan a recorded launch must be ready for any
+        step (and what it was given is never replaced, no step needs more); another knows whether this one's items
+        are cut."""
+        if self._split_ctas:
+            if not self._cutting:
+                self._start_cutting()
+            if self.replayable and torch.cuda.is_current_stream_capturing():
+                return self._workspace_of(2 * self._split_ctas)
+        return self._workspace_of(self._num_partials)
 
     def _build(self, cu_seqlens_q, seqlens_kv, causal_base) -> None:
         lib = _lib.load()
@@ -610,12 +653,8 @@ class PrefillPlan:
                                    self.host.data_ptr(), self.host.numel() * 4, ctypes.byref(self.info))
         _lib.check(rc, "b200_prefill_plan")
         self._num_partials = 0
-        if self._split_ctas:
-            partials = ctypes.c_int(0)
-            rc = lib.b200_prefill_split(self.host.data_ptr(), self.host.numel() * 4, self._split_ctas,
-                                        ctypes.byref(self.info), ctypes.byref(partials))
-            _lib.check(rc, "b200_prefill_split")
-            self._num_partials = partials.value
+        if self._cutting:
+            self._cut()
 
     def _upload(self, used: int) -> None:
         self.dev[:used].copy_(self.host[:used], non_blocking=True)
@@ -705,8 +744,7 @@ def paged_prefill_gqa_fp8(q: torch.Tensor, key_cache: torch.Tensor, value_cache:
         lse_out)
     t, n_q, _ = q.shape
     rows, cols = block_table.shape
-    # a recorded launch must be ready for any step; another knows whether this one's items are cut
-    workspace = plan.workspace if plan._num_partials or plan.replayable and torch.cuda.is_current_stream_capturing() else None
+    workspace = plan._launch_workspace()
     _call_on(index, "b200_paged_prefill_gqa_fp8", q.data_ptr(), q.stride(0), key_cache.data_ptr(),
              value_cache.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(), num_blocks, block_size,
              block_table.data_ptr(), block_table.stride(0), rows, cols, plan.dev.data_ptr(),

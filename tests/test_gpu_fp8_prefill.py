@@ -499,3 +499,52 @@ def test_many_small_weights_beside_a_key_that_carries_the_row(mass, sink_v, n, q
     err = (got.double() - want).abs()
     assert (err <= tol).all(), float((err / tol).max())
     torch.testing.assert_close(lse.cpu().double(), want_lse, rtol=2.0 ** -16, atol=2.0 ** -14)
+
+
+def test_a_plan_is_cut_and_has_a_workspace_when_that_is_needed():
+    """Neither for the 16-bit kernel; from the first launch over an 8-bit cache on, with room for what the step needs in an
+    eager launch and for what any step needs in a recorded one."""
+    from auto_infer_b200 import ops
+    c = _case(45, [9000, 50], [4, 12], 8, 1, 64)
+    dev = [x.cuda() for x in c[:6]]
+    kc = (dev[1].float() * dev[3][:, None, :, None]).to(torch.bfloat16)
+    vc = (dev[2].float() * dev[4][:, None, :, None]).to(torch.bfloat16)
+    want, lse = _run(*c)
+    _check(want, lse, *c)
+    record = 128 * 129 * 4
+    for capacity in (None, 16):
+        before = torch.cuda.memory_allocated()
+        plan = ops.PrefillPlan(c[6], c[7], 8, 1, "cuda", min_rows=0, capacity_tokens=capacity, capacity_seqs=capacity and 2)
+        wide = ops.paged_prefill_gqa(dev[0], kc, vc, dev[5], plan, c[8])
+        if capacity:
+            plan.refill(c[6], c[7])
+            assert torch.equal(ops.paged_prefill_gqa(dev[0], kc, vc, dev[5], plan, c[8]), wide)
+        assert not plan.host[4:8].any() and torch.cuda.memory_allocated() - before < record
+        for _ in range(2):
+            assert torch.equal(ops.paged_prefill_gqa_fp8(*dev, plan, c[8]).cpu(), want)
+            assert plan.host[4] > 0 and 2 * record <= plan.workspace.numel() < ops.sm_count() * record
+            assert torch.equal(ops.paged_prefill_gqa(dev[0], kc, vc, dev[5], plan, c[8]), wide)
+            if capacity:
+                plan.refill(c[6], c[7])
+                assert plan.host[4] > 0
+    asked = ops.PrefillPlan(c[6], c[7], 8, 1, "cuda", min_rows=0, split_ctas=ops.sm_count())
+    assert torch.equal(asked.host[:asked.info.plan_ints], plan.host[:plan.info.plan_ints])
+    for first in (True, False):                          # the recorded launch is the plan's first over an 8-bit cache
+        if first:
+            plan = ops.PrefillPlan(c[6], c[7], 8, 1, "cuda", min_rows=0, capacity_tokens=16, capacity_seqs=2)
+        graph, out = torch.cuda.CUDAGraph(), torch.empty_like(dev[0])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            ops.paged_prefill_gqa_fp8(*dev, plan, c[8], out=out)
+        assert plan._workspace.numel() >= 2 * ops.sm_count() * record
+        graph.replay()
+        lse = attention(*c)[1].float()
+        _check(out.cpu(), lse, *c)
+        held = plan._workspace.data_ptr()
+        for _ in range(2):
+            plan.refill(c[6], c[7])
+            out.fill_(3.0)
+            graph.replay()
+            assert torch.equal(out.cpu(), want)
+            assert torch.equal(ops.paged_prefill_gqa_fp8(*dev, plan, c[8]).cpu(), want) and plan._workspace.data_ptr() == held
+    assert ops.read_status("cuda") == 0

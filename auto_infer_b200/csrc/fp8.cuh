@@ -75,6 +75,13 @@ __device__ __forceinline__ float fast_log2(float x) {
 __device__ __forceinline__ void cp_async_f32(float* dst, const float* src, bool have) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(have ? 4 : 0) : "memory");
 }
+// Waits for a phase that completes by itself, of copies or matrix products that are under way, whatever the CTA's abort flag
+// says: a CTA that gives up must not leave while they write to its memory.  At most 2^20 tries of a microsecond or so.
+__device__ __forceinline__ void mbar_wait_landed(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t left = 1u << 20; left && !mbar_try_wait(bar, parity); --left) {
+  }
+}
 // One of the barrier's expected arrivals, made when this thread's cp.async copies so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");

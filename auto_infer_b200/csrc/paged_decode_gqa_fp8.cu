@@ -366,6 +366,7 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       const int s = it % kF8Stages;
       const uint32_t ph = (it / kF8Stages) & 1u;
       mbar_wait_bounded(&sm.empty[s], ph ^ 1u, abort_flag, p.status);
+      if (__any_sync(0xffffffffu, *abort_flag)) break;      // the stage may still be in use: nothing more is loaded
       if (lane == 0) mbar_arrive_expect_tx(&sm.full[s], kF8StageBytes);
       __syncwarp();
       if (lane < nbox) {
@@ -388,12 +389,13 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
       ++it;
       ++w.tile;
     }
-    // drain: do not leave while copies may still land in this CTA's shared memory
+    // drain: do not leave while copies may still land in this CTA's shared memory.  `it` is past the last tile, or the first
+    // tile of this group that was not loaded.
     if (lane == 0) {
       const uint32_t mine = (it + kF8Groups - 1 - grp) / kF8Groups;      // tiles this warp has loaded
       for (uint32_t k = 0; k < (uint32_t)(kF8Stages / kF8Groups) && k < mine; ++k) {
         const uint32_t j = (mine - 1 - k) * kF8Groups + grp;
-        mbar_wait_bounded(&sm.full[j % kF8Stages], (j / kF8Stages) & 1u, abort_flag, p.status);
+        mbar_wait_landed(&sm.full[j % kF8Stages], (j / kF8Stages) & 1u);
       }
     }
     return;

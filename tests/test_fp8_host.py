@@ -270,3 +270,26 @@ def test_backends_over_different_caches_do_not_share_a_contexts_plans(monkeypatc
             assert list(pools[n].values()) == [got[n]]
         assert metadata.cached_step_metadata(ctx, 8, 2, 128, "cpu") is got[2]
         assert len(built) == 2
+
+
+def _producer(name):
+    """The loads of a kernel's producer and the waits it leaves by, as two pieces of source."""
+    import os
+    from auto_infer_b200 import build
+    text = open(os.path.join(build.CSRC, name)).read()
+    text = text[text.index("tma_prefetch_desc(&v_map)"):]
+    loop, drain = text.split("// drain: ", 1)
+    return loop, drain[:drain.index("return;" if "decode" in name else "} else if")]
+
+
+@pytest.mark.parametrize("name, waits", [("paged_decode_gqa_fp8.cu", 1)])
+def test_a_producer_that_gives_up_loads_nothing_more_and_waits_for_what_it_has_loaded(name, waits):
+    """Read from the source, as no wait of a sound kernel runs out: between a producer's wait for a free stage and the load
+    into it stands the way out of the loop, and the waits before it leaves pass by no abort flag."""
+    import re
+    loop, drain = _producer(name)
+    steps = re.findall(r"mbar_wait_\w+\(&sm\.\w*empty\[s\w?\]|__any_sync\(0xffffffffu, \*abort_flag\)\) break|"
+                       r"mbar_arrive_expect_tx|tma_load_4d", loop)
+    kinds = "".join("w" if "wait" in s else "b" if "break" in s else "l" for s in steps)
+    assert re.fullmatch("(wbl+){%d}" % waits, kinds), kinds
+    assert "mbar_wait_landed" in drain and "abort_flag" not in drain and "mbar_wait_bounded" not in drain

@@ -103,6 +103,7 @@ struct __align__(1024) Prefill8Smem {
   uint64_t l_empty;                        // and read
   uint64_t q_full[2];                      // per item parity: the Q terms and row factors are staged
   uint64_t q_empty[2];                     // all S MMAs of the item have run
+  uint64_t mma_idle[2];                    // end of the CTA: all MMAs of the S and the P V issuer have run
   uint64_t item_full[2];                   // work-queue hand-off: producer warp -> the other roles
   uint64_t item_empty[2];
   alignas(16) PrefillPiece next_rec[2];    // the mailbox carries the whole record (read as int4)
@@ -143,23 +144,28 @@ __host__ __device__ constexpr uint32_t umma_idesc_type0(int m, int n, bool b_mn_
 // flag goes up: every later wait returns at once, so control flow stays uniform, the kernel drains to its end and reports
 // B200_STATUS_WAIT_TIMEOUT there.  A dozen instructions: it stands at every wait of loops that together have to stay in the
 // instruction cache.
-__device__ __forceinline__ void mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t abort_at) {
+// Returns whether the phase has completed.
+__device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t abort_at) {
+  uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .u32 left, gone;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 left, gone;\n\t"
       "mov.u32 left, 0x100000;\n"
       "again:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
-      "@p bra through;\n\t"
-      "ld.volatile.shared.u32 gone, [%2];\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\t"
+      "@q bra through;\n\t"
+      "ld.volatile.shared.u32 gone, [%3];\n\t"
       "setp.ne.u32 p, gone, 0;\n\t"
       "@p bra through;\n\t"
       "sub.u32 left, left, 1;\n\t"
       "setp.ne.u32 p, left, 0;\n\t"
       "@p bra again;\n\t"
-      "st.volatile.shared.u32 [%2], 1;\n"
-      "through:\n\t}"
-      ::"r"(smem_u32(bar)), "r"(parity), "r"(abort_at)
+      "st.volatile.shared.u32 [%3], 1;\n"
+      "through:\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(abort_at)
       : "memory");
+  return ok != 0;
 }
 
 // Shared-memory matrix descriptor (128-byte swizzle) in two parts: the word with the address, and the rest.
@@ -216,6 +222,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
       mbar_init(&sm.m_ready[b], 128);
       mbar_init(&sm.q_full[b], kP8ConvertThreads);
       mbar_init(&sm.q_empty[b], 1);
+      mbar_init(&sm.mma_idle[b], 1);
       mbar_init(&sm.item_full[b], 1);
       mbar_init(&sm.item_empty[b], kP8SoftmaxThreads + 2 + kP8ConvertThreads);   // all consumers of the mailbox
     }
@@ -259,7 +266,7 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
         tma_prefetch_desc(&k_map);
         tma_prefetch_desc(&v_map);
       }
-      uint32_t it = 0;
+      uint32_t it = 0, k_loaded = 0, v_loaded = 0;       // K (and scales), V: tiles whose copies have been issued
       const int nbox = p.boxes_per_tile;
       auto draw = [&](uint32_t k) -> int {
         int idx = -1;
@@ -319,9 +326,9 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             ids[0] = bid;
             const int b = __shfl_sync(0xffffffffu, bid, (lane * groups_per_box) & 31);
             const int sk = itx % kP8KStages;
-            mbar_wait_limited(&sm.k_empty[sk], ((itx / kP8KStages) & 1u) ^ 1u, abort_at);
-            if (lane == 0) mbar_arrive_expect_tx(&sm.k_full[sk], kP8TileBytes);
-            __syncwarp();
+            const bool stage_free = mbar_wait_limited(&sm.k_empty[sk], ((itx / kP8KStages) & 1u) ^ 1u, abort_at);
+            if (lane == 0 && stage_free) mbar_arrive_expect_tx(&sm.k_full[sk], kP8TileBytes);
+            if (!__all_sync(0xffffffffu, stage_free)) break;       // a wait has run out: nothing more is loaded
             if (lane < nbox)                         // a page outside the pool: TMA fills zeros
               tma_load_4d(sm.k[sk] + box_row * kFp8HeadDim, &k_map, &sm.k_full[sk], 0, item.kv_head,
                           ((first_of(item) + step) * kPfTile + box_row) & (p.block_size - 1), b < 0 ? p.num_blocks : b);
@@ -335,37 +342,40 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
               cp_async_f32(&sm.tile_scale[sl][1][lane], p.scale_of[1] + at, bid >= 0);
             }
             cp_async_arrive(&sm.scale_full[sl]);
+            ++k_loaded;
           }
           if (step >= kP8KLead && n > 0) {
             const int tile = step - kP8KLead;
             const uint32_t itx = it + tile;
             const int b = __shfl_sync(0xffffffffu, ids[kP8KLead], (lane * groups_per_box) & 31);
             const int sv = itx % kP8VStages;
-            mbar_wait_limited(&sm.v_empty[sv], ((itx / kP8VStages) & 1u) ^ 1u, abort_at);
-            if (lane == 0) mbar_arrive_expect_tx(&sm.v_full[sv], kP8TileBytes);
-            __syncwarp();
+            const bool stage_free = mbar_wait_limited(&sm.v_empty[sv], ((itx / kP8VStages) & 1u) ^ 1u, abort_at);
+            if (lane == 0 && stage_free) mbar_arrive_expect_tx(&sm.v_full[sv], kP8TileBytes);
+            if (!__all_sync(0xffffffffu, stage_free)) break;
             if (lane < nbox)
               tma_load_4d(sm.v[sv] + box_row * kFp8HeadDim, &v_map, &sm.v_full[sv], 0, item.kv_head,
                           ((first_of(item) + tile) * kPfTile + box_row) & (p.block_size - 1), b < 0 ? p.num_blocks : b);
+            ++v_loaded;
           }
           __syncwarp();
         }
+        if (__any_sync(0xffffffffu, *abort_flag)) break;
         it += n;
         item = sm.next_rec[k & 1u];                  // not overwritten before this warp draws item k + 2
       }
       // drain: nothing may still be landing when the CTA leaves
       if (lane == 0) {
-        for (uint32_t k = 0; k < (uint32_t)kP8KStages && k < it; ++k) {
-          const uint32_t j = it - 1 - k;
-          mbar_wait_limited(&sm.k_full[j % kP8KStages], (j / kP8KStages) & 1u, abort_at);
+        for (uint32_t k = 0; k < (uint32_t)kP8KStages && k < k_loaded; ++k) {
+          const uint32_t j = k_loaded - 1 - k;
+          mbar_wait_landed(&sm.k_full[j % kP8KStages], (j / kP8KStages) & 1u);
         }
-        for (uint32_t k = 0; k < (uint32_t)kP8VStages && k < it; ++k) {
-          const uint32_t j = it - 1 - k;
-          mbar_wait_limited(&sm.v_full[j % kP8VStages], (j / kP8VStages) & 1u, abort_at);
+        for (uint32_t k = 0; k < (uint32_t)kP8VStages && k < v_loaded; ++k) {
+          const uint32_t j = v_loaded - 1 - k;
+          mbar_wait_landed(&sm.v_full[j % kP8VStages], (j / kP8VStages) & 1u);
         }
-        for (uint32_t k = 0; k < (uint32_t)kP8ScaleSlots && k < it; ++k) {
-          const uint32_t j = it - 1 - k;
-          mbar_wait_limited(&sm.scale_full[j % kP8ScaleSlots], (j / kP8ScaleSlots) & 1u, abort_at);
+        for (uint32_t k = 0; k < (uint32_t)kP8ScaleSlots && k < k_loaded; ++k) {
+          const uint32_t j = k_loaded - 1 - k;
+          mbar_wait_landed(&sm.scale_full[j % kP8ScaleSlots], (j / kP8ScaleSlots) & 1u);
         }
       }
     } else if (warp == 9) {
@@ -403,6 +413,8 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
             if (tile == n_tiles - 1) umma_commit(&sm.q_empty[qb]);   // the Q terms may be overwritten
           }
         }
+        umma_commit(&sm.mma_idle[0]);
+        mbar_wait_landed(&sm.mma_idle[0], 0);
       }
       __syncwarp();
     } else if (warp == 10) {
@@ -439,6 +451,8 @@ paged_prefill_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid
           }
           umma_commit(&sm.o_done);
         }
+        umma_commit(&sm.mma_idle[1]);
+        mbar_wait_landed(&sm.mma_idle[1], 0);
       }
       __syncwarp();
     }

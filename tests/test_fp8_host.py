@@ -282,14 +282,27 @@ def _producer(name):
     return loop, drain[:drain.index("return;" if "decode" in name else "} else if")]
 
 
-@pytest.mark.parametrize("name, waits", [("paged_decode_gqa_fp8.cu", 1)])
+@pytest.mark.parametrize("name, waits", [("paged_decode_gqa_fp8.cu", 1), ("paged_prefill_gqa_fp8.cu", 2)])
 def test_a_producer_that_gives_up_loads_nothing_more_and_waits_for_what_it_has_loaded(name, waits):
     """Read from the source, as no wait of a sound kernel runs out: between a producer's wait for a free stage and the load
-    into it stands the way out of the loop, and the waits before it leaves pass by no abort flag."""
+    into it stands the way out of the loop (a barrier is armed behind it, or by a lane that saw the stage free), and the
+    waits before it leaves pass by no abort flag."""
     import re
     loop, drain = _producer(name)
     steps = re.findall(r"mbar_wait_\w+\(&sm\.\w*empty\[s\w?\]|__any_sync\(0xffffffffu, \*abort_flag\)\) break|"
+                       r"!__all_sync\(0xffffffffu, stage_free\)\) break|stage_free\) mbar_arrive_expect_tx|"
                        r"mbar_arrive_expect_tx|tma_load_4d", loop)
-    kinds = "".join("w" if "wait" in s else "b" if "break" in s else "l" for s in steps)
-    assert re.fullmatch("(wbl+){%d}" % waits, kinds), kinds
-    assert "mbar_wait_landed" in drain and "abort_flag" not in drain and "mbar_wait_bounded" not in drain
+    kinds = "".join("w" if "wait" in s else "b" if "break" in s else "a" if s.startswith("stage_free") else "l" for s in steps)
+    assert re.fullmatch("(wa?bl+){%d}b?" % waits, kinds), kinds
+    assert "mbar_wait_landed" in drain and "abort" not in drain and not re.search("mbar_wait_(bounded|limited)", drain)
+
+
+def test_tensor_memory_is_not_given_back_under_matrix_products():
+    """Each of the two issuing warps ends with a commit of its own and waits for it whatever the abort flag says."""
+    import os
+    import re
+    from auto_infer_b200 import build
+    text = open(os.path.join(build.CSRC, "paged_prefill_gqa_fp8.cu")).read()
+    ends = [m.start() for m in re.finditer(r"umma_commit\(&sm\.mma_idle\[(\d)\]\);\s+mbar_wait_landed\(&sm\.mma_idle\[\1\], 0\);", text)]
+    roles = [text.index(s) for s in ("} else if (warp == 9) {", "} else if (warp == 10) {", "} else if (warp < 8) {")]
+    assert len(ends) == 2 and roles[0] < ends[0] < roles[1] < ends[1] < roles[2] < text.index("tmem_dealloc")

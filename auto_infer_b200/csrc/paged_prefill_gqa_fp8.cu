@@ -141,10 +141,10 @@ __host__ __device__ constexpr uint32_t umma_idesc_type0(int m, int n, bool b_mn_
 }
 // Waits for a phase of an mbarrier, at most 2^20 tries of up to about 1.5 us each, which is how long the unit suspends a
 // thread by default (a longer hint wakes it later: 582 us instead of 568 on an 8192-token prompt).  Then the CTA's abort
-// flag goes up: every later wait returns at once, so control flow stays uniform, the kernel drains to its end and reports
-// B200_STATUS_WAIT_TIMEOUT there.  A dozen instructions: it stands at every wait of loops that together have to stay in the
-// instruction cache.
-// Returns whether the phase has completed.
+// flag goes up: every later wait returns at once, so control flow stays uniform, nothing more is loaded, the copies and matrix
+// products under way are waited for (mbar_wait_landed) and the kernel reports B200_STATUS_WAIT_TIMEOUT at its end.  A dozen
+// instructions: it stands at every wait of loops that together have to stay in the instruction cache.  Returns whether the
+// phase has completed.  (The producer goes by that: its reading the flag for each load took 547 us instead of 527.)
 __device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t abort_at) {
   uint32_t ok;
   asm volatile(

@@ -452,7 +452,8 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
     if (atomicAdd(&mg->arrivals, 1) == n_parts - 1) {
       mg->arrivals = 0;                           // ready for the next launch on this plan
       __threadfence();                            // the other CTAs' records are visible from here on
-      if (sm.merge_count < kMaxDeferred) {
+      if (mg->part_end > p.max_partials) {        // not all of them found room: there is nothing to merge
+      } else if (sm.merge_count < kMaxDeferred) {
         sm.merge_list[sm.merge_count] = multi_idx;
         sm.merge_count = sm.merge_count + 1;
       } else if (p.status) {                      // the planner never gives a CTA this many cut pieces
@@ -722,11 +723,10 @@ paged_decode_gqa_fp8_kernel(const __grid_constant__ CUtensorMap k_map, const __g
         if ((t & 31) == 0) rec[kMaxRows * kHeadDim + row] = lse_r[h];
       }
     }
-    if (!record_fits) {                                        // workspace, q or out smaller than the plan needs
-      if (t == 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);
-    } else if (!item.direct) {
-      pending_multi = item.multi_idx;
-    }
+    if (!record_fits && t == 0 && p.status) atomicOr(p.status, B200_STATUS_BAD_LAUNCH);   // workspace, q or out too small
+    // Also a record that found no room is counted, or the pair's counter would be off for the next launch on this plan.
+    // (Rows outside q leave out all pieces of a pair, and nothing is to be merged then.)
+    if (!item.direct && rows > 0) pending_multi = item.multi_idx;
     // The next item's first write to red_m / red_o comes after barrier (3) above, and its first write
     // to red_l and to the slots after its own barrier (1), which no thread passes before it has
     // finished the reads of this item.

@@ -334,3 +334,33 @@ def test_many_small_weights_beside_a_key_that_carries_the_row(mass, sink_v, n, q
     err = (got.double() - want).abs()
     assert (err <= tol).all(), float((err / tol).max())
     torch.testing.assert_close(lse.double(), want_lse, rtol=2.0 ** -18, atol=2.0 ** -16)
+
+
+@pytest.mark.parametrize("share", [0.0, 0.3, 0.5, 0.9])
+def test_a_workspace_that_is_too_small_spoils_its_own_launch_only(share):
+    """The replayable launch cannot know what the plan needs: it says so in the status word, puts the counters of the cut pairs
+    back to zero all the same, and the plan gives the right rows with the workspace it asks for."""
+    from auto_infer_b200 import _lib, ops
+    c = _case(46, [9000, 5000, 40], [1, 2, 1], 8, 2, 64)
+    q, kc, vc, ks, vs, table = [x.cuda() for x in c[:6]]
+    plan = ops.DecodePlan(c[6], c[7], 8, 2, "cuda", capacity_seqs=3)
+    want = ops.paged_decode_gqa_fp8(q, kc, vc, ks, vs, table, plan, c[8])
+    record = (16 * 128 + 16) * 4
+    assert plan.info.num_partials > 8
+    small = int(plan.info.num_partials * share) * record
+    lib, out, lse = _lib.load(), torch.empty_like(q), torch.empty(4, 8, device="cuda")
+    for nbytes, status in ((small, _lib.STATUS_BAD_LAUNCH), (plan.workspace.numel(), 0), (small, _lib.STATUS_BAD_LAUNCH),
+                           (small, _lib.STATUS_BAD_LAUNCH), (plan.workspace.numel(), 0), (plan.workspace.numel(), 0)):
+        out.fill_(3.0)
+        plan.workspace.view(torch.float32).fill_(math.nan)   # no record of an earlier launch is left
+        assert lib.b200_paged_decode_gqa_fp8(
+            q.data_ptr(), q.stride(0), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), kc.shape[0], 64,
+            table.data_ptr(), table.stride(0), *table.shape, plan.dev.data_ptr(), None, plan.num_ctas, 4, 8, 2, 128, c[8],
+            plan.workspace.data_ptr(), nbytes, out.data_ptr(), 0, lse.data_ptr(), ops.status_word("cuda").data_ptr(),
+            torch.cuda.current_stream().cuda_stream) == 0
+        assert ops.read_status("cuda") == status
+        pairs, at = int(plan.host[4]), int(plan.host[7])
+        assert pairs == 4 and not plan.dev[at:at + 8 * pairs].view(pairs, 8)[:, 5].any()
+        if not status:
+            assert torch.equal(out, want)
+    _check(out.cpu(), lse.cpu(), *c)

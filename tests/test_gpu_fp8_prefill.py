@@ -548,3 +548,26 @@ def test_a_plan_is_cut_and_has_a_workspace_when_that_is_needed():
             assert torch.equal(out.cpu(), want)
             assert torch.equal(ops.paged_prefill_gqa_fp8(*dev, plan, c[8]).cpu(), want) and plan._workspace.data_ptr() == held
     assert ops.read_status("cuda") == 0
+
+
+@pytest.mark.parametrize("max_ctas", [1, 2, 3])
+@pytest.mark.parametrize("split", [0, None])
+def test_every_launch_of_items_with_and_without_rows_gives_the_same_bits(split, max_ctas):
+    """Output and sums of each of many launches, whole items and cut ones, on few CTAs, where a warp that has no row in one item
+    has some in the next: all like the first launch's, and that one right."""
+    from auto_infer_b200 import ops
+    q_lens = [3, 128, 1, 128, 33, 128, 64, 2, 128, 5, 97, 128, 1, 1, 128, 40]
+    lens = [900, 128, 130, 300, 400, 1000, 64, 513, 257, 5, 200, 700, 1, 260, 129, 380]
+    for bs in (32, 128):
+        c = _case(17, lens, q_lens, 1, 1, bs)
+        dev = [x.cuda() for x in c[:6]]
+        plan = ops.PrefillPlan(c[6], c[7], 1, 1, "cuda", min_rows=0, split_ctas=split)
+        calls = []
+        for _ in range(30):
+            lse = torch.full((c[6][-1], 1), 7.0, device="cuda")
+            out = torch.full_like(dev[0], 3.0)
+            ops.paged_prefill_gqa_fp8(*dev, plan, c[8], out=out, lse_out=lse, max_ctas=max_ctas)
+            calls.append((out, lse))
+        _check(*[x.cpu() for x in calls[0]], *c)
+        assert all(torch.equal(out, calls[0][0]) and torch.equal(lse, calls[0][1]) for out, lse in calls)
+    assert ops.read_status("cuda") == 0

@@ -27,14 +27,18 @@
 // Tensor-bound: flops = 4 * 128 * sum over rows of visible keys; 1024 tensor cycles and 1024 cycles of exponentials for a
 // tile of 128 x 128.  A tile takes about 1850 cycles: each group's chain scores -> maximum -> weights -> P is about 3700
 // long, two of them run, and a softmax warp issues an instruction in about three cycles.  Where an item ends, O has
-// to be read before the next item's first P V.  Measured (32 query heads, 8 kv heads): 520 us on an 8192-token prompt (1057
-// TFLOP/s), 106 us on four 512-token chunks over cached prefixes, 38 us on 16 drafts of 5 tokens over 512 to 4096
-// tokens (42 uncut).  Where few items meet many SMs the plan cuts them along the keys (b200_prefill_split) and a second kernel joins
-// the pieces: 81 us instead of 985 on 16 rows over 131072 tokens, 85 instead of 262 on 2 x 64 rows over 32768, 53 instead
-// of 69 on 16 drafts over 2048 to 8192.  What else was tried: both groups on row tiles of their own with one K / V stream (620 us: the
-// instruction footprint of two O rescales), the groups' exponential sections kept apart by a barrier (799 us against 742 at
-// the time).  All roles' loops share the SM's instruction cache, so each piece of code is instantiated once and outer
-// loops are not unrolled: from 85 KB of code to 64 KB, with the waits in line, took 742 us to 581.
+// to be read before the next item's first P V.  Measured (32 query heads, 8 kv heads; replayed graphs): 527 us on an
+// 8192-token prompt (1043 TFLOP/s; about 590 in a long loop of calls, where the clock falls), 105 to 110 us on four 512-token
+// chunks over cached prefixes, 37 us on 16 drafts of 5 tokens over 512 to 4096 tokens (42 uncut); a 4096-token prompt takes
+// 158 us over pages of 128, 194 over pages of 64 or 32 and 212 over pages of 16 (eight pairs of scales a tile, and
+// spills).  The kernel over a 16-bit cache is faster on prompts (518, 93 and 134 to 162 us): the 8-bit one is for the
+// cache's size, not for these.  Where few items meet many SMs the plan cuts them along the keys (b200_prefill_split) and a
+// second kernel joins the pieces: 83 us instead of 982 on 16 rows over 131072 tokens, 89 instead of 265 on 2 x 64 rows over
+// 32768, 62 instead of 73 on 16 drafts over 2048 to 8192.  What else was tried: both groups on row tiles of their own with
+// one K / V stream (620 us: the instruction footprint of two O rescales), the groups' exponential sections kept apart by a
+// barrier (799 us against 742 at the time).  All roles' loops share the SM's instruction cache, so each piece of code is
+// instantiated once and outer loops are not unrolled: from 85 KB of code to 64 KB, with the waits in line, took 742 us to
+// 581; the four variants have 53 to 57 KB now.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

@@ -20,7 +20,7 @@ _ATTR = "_b200_step_meta"
 # CTAs together move (GB/s), what one moves beside the wide-query kernel (GB/s), and how long one SM
 # works on a 128 x 128 tile of the wide-query kernel (us).  The 8-bit kernels' figures are
 # fits to 24 to 120 SMs each on five mixes of 16 to 128 decode rows with 256 to 8192 new prompt tokens; of those,
-# side by side wins most on 60 decode rows beside one 256-token chunk (130 us, 156 one after the other).
+# side by side wins most on 60 decode rows beside one 256-token chunk (118 to 126 us, 146 one after the other).
 _RATES = {2: (6450.0, 53.0, 1.26), 1: (5500.0, 48.0, 1.15)}
 _DECODE_FIXED_US, _PREFILL_FIXED_US = 6.0, 4.0
 

@@ -255,12 +255,17 @@ int b200_paged_decode_gqa_write(const void* q, int64_t q_stride,
  * the launch is the replayable one (grid num_ctas, counts read from the plan).
  *   block_size a power of two from 16 to 1024; q 8-byte aligned, q_stride a multiple
  *       of 4 elements
- *   scales: positive finite numbers, any, not only powers of two
+ *   scales of the pages: positive finite numbers, any, not only powers of two (a page
+ *       whose scale is 0 reads as zeros); scale: any finite number, of either sign
  *   table_rows, table_cols: entries of block_table; a sequence or page past them
  *       reads as zeros and sets B200_STATUS_BAD_BLOCK
  *   num_tokens: rows of q and out; items of the plan past them are left out and set
  *       B200_STATUS_BAD_LAUNCH
- * Cache rows past a sequence's kv_len may hold any codes. */
+ *   workspace: with info == NULL a plan that needs more sets B200_STATUS_BAD_LAUNCH and
+ *       leaves the rows of the pairs concerned unwritten
+ * Cache rows past a sequence's kv_len may hold any codes; a NaN code of V in a row that the
+ * last query row of a sequence sees and its first does not makes NaN of that column for all
+ * query rows of the sequence, as a matrix product with a zero weight does. */
 int b200_paged_decode_gqa_fp8(const void* q, int64_t q_stride,
                               const void* key_cache, const void* value_cache,
                               const float* key_scale, const float* value_scale,
@@ -364,7 +369,7 @@ int b200_prefill_split(int32_t* plan_host, size_t plan_bytes, int num_ctas,
  * plan is known not to be cut (the launch then costs less); a plan that needs more than it holds
  * sets B200_STATUS_BAD_LAUNCH; max_ctas > 0 keeps it to that many SMs as _on does; with
  * info == NULL the launch is the replayable one.  block_size, table_rows,
- * table_cols, num_tokens and the scales as b200_paged_decode_gqa_fp8.  Cache rows
+ * table_cols, num_tokens, scale and the pages' scales as b200_paged_decode_gqa_fp8.  Cache rows
  * past a sequence's kv_len may hold any codes; a NaN code of V in a row that one
  * query row of a 128-row item sees makes NaN of that column for all rows of the item
  * that share its 128-token tile, as a matrix product with a zero weight does. */

@@ -169,6 +169,8 @@ int b200_decode_plan(const int32_t* cu_seqlens_q_host, const int32_t* seqlens_kv
  *             geometry), 16-byte aligned
  *   out: (T, Hq, 128) bf16 when out_is_f32 == 0, fp32 otherwise (the fp32 form
  *        is one context-parallel rank's partial); lse_out (T, Hq) fp32 or NULL
+ *   scale: a positive finite number, here and in b200_paged_prefill_gqa (these kernels
+ *        mask and take maxima before they multiply by it)
  * Mask: bottom-right causal (sparse_mode 3 of the vendor op).  Cache rows past a
  * sequence's kv_len (the unwritten tail of its last page) are never read into the
  * arithmetic: they may hold any bytes. */
